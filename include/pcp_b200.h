@@ -34,6 +34,9 @@ typedef struct pcpb_buffer pcpb_buffer;
 
 /* Element types, numbered like DType in src/core/tensor.zig:9-62. */
 enum pcpb_dtype { PCPB_F32 = 0, PCPB_F64 = 1, PCPB_F16 = 2, PCPB_BF16 = 3, PCPB_I32 = 4, PCPB_I64 = 5, PCPB_BOOL = 6 };
+/* Code types of a quantised KV cache (no counterpart in the reference): signed 8-bit integers, and 8-bit floats with four
+ * exponent and three fraction bits. */
+enum pcpb_code_dtype { PCPB_I8 = 16, PCPB_E4M3 = 17 };
 
 enum pcpb_status {
   PCPB_OK = 0,
@@ -379,6 +382,113 @@ int pcpb_rollout_generate(pcpb_rollout* r, const int64_t* prompts, const int* pr
 /* Logits (as f32) of sequence `row` at the most recent step, for checks. */
 int pcpb_rollout_read_logits(pcpb_rollout* r, int row, float* dst, size_t n);
 long long pcpb_rollout_launch_count(const pcpb_rollout* r);
+
+/* ---- decode operators on caller-owned device memory ----------------------------------------------------------
+ * What a decoding loop needs beside the rollout engine when it holds its cache in 8 bits and checks several drafted
+ * tokens per step: rows written into a paged cache and read back, attention of a tree of drafted tokens over that cache,
+ * and the choice of the accepted ones.  The reference's engine keeps a dense cache, decodes one token per call and samples
+ * on the host (src/nodes/workers/generation_engine.zig:174-332, src/core/math.zig:21-73); the page layout is the rollout
+ * engine's.  Rules common to the four calls:
+ *   - every pointer in a call is device memory of ONE device, which becomes the current one for the call; host memory and
+ *     memory of another device are refused (PCPB_E_INVALID).  `stream` is a cudaStream_t of that device, NULL its default
+ *     stream.  A call enqueues its kernels and returns; it allocates nothing, keeps nothing and may be captured.
+ *   - rows and pages start on 16-byte boundaries and strides are counted in elements; others are refused.
+ *   - lengths, page numbers and tree links live on the device and cannot be refused on the host.  The kernels check each
+ *     before they use it, leave out what is out of range and set the PCPB_OPS_* bit in *status (optional, OR-ed, never
+ *     cleared).
+ *   - two calls at once may share every input, but not an output, a workspace or pages that one of them writes.
+ *   - err (optional) receives the reason of a refusal. */
+#define PCPB_OPS_BAD_PAGE 1      /* a block-table entry outside the cache: its rows were not written / not attended / read as 0 */
+#define PCPB_OPS_BAD_LENGTH 2    /* a negative or too large length, start or row number: clipped to what there is */
+#define PCPB_OPS_BAD_TREE 4      /* a parent that does not come before its child: the node counts as a root */
+#define PCPB_OPS_NO_CHOICE 8     /* logits without a finite largest value, or a token outside the vocabulary */
+
+/* One layer's paged cache: page p holds rows [n_kv_head][page_tokens][head_dim] at k + p * page_stride.  Position t of
+ * sequence b is row t % page_tokens of page block_table[b * max_pages + t / page_tokens].  dtype PCPB_BF16 holds the rows
+ * as they are; PCPB_E4M3 and PCPB_I8 hold codes c and per row and head one f32 scale a, value a * c:
+ *   a = max(largest magnitude of the row / Q, 2^-126), Q = 448 (e4m3) or 127 (i8);  c = x / a (f32) rounded to nearest even.
+ * A row with an infinity or a NaN gets scale NaN, so that all of it reads back as NaN. */
+typedef struct pcpb_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;        /* [page][n_kv_head][page_tokens]; NULL for PCPB_BF16 */
+  const int32_t* block_table;      /* [batch][max_pages] */
+  long long page_stride;           /* elements from page to page in k and v; 0: n_kv_head * page_tokens * head_dim */
+  long long scale_stride;          /* the same in k_scale and v_scale; 0: n_kv_head * page_tokens */
+  int dtype, n_pages, n_kv_head, head_dim, page_tokens, batch, max_pages;     /* head_dim 32, 64 or 128 */
+} pcpb_kv_cache;
+
+/* Rows that go into or come out of a cache.  The entries of sequence b are [cu_rows[b], cu_rows[b + 1]); entry e is the
+ * position pos0[b] + e - cu_rows[b] and the row `index[e]` of k and v (index NULL: row e; negative: no row, the entry is
+ * left out).  Entries from cu_rows[batch] on are left out too: nothing of theirs is touched. */
+typedef struct pcpb_kv_rows {
+  void *k, *v;                     /* PCPB_BF16 or PCPB_F32, element [row][head][i] at row * k_row + head * k_head + i */
+  long long k_row, k_head, v_row, v_head;
+  const int32_t *cu_rows, *pos0, *index;
+  int dtype, n_rows, n_entries;    /* rows of k and v; entries the call may look at */
+} pcpb_kv_rows;
+/* Writes rows into the cache, quantised on the way (one pass: every row is read once).  Two entries for one slot (two
+ * sequences whose block tables share the page, or an index list that names a page twice) leave either row or a mix of both
+ * there. */
+int pcpb_op_kv_write(void* stream, const pcpb_kv_cache* cache, const pcpb_kv_rows* rows, int32_t* status, char* err, size_t err_cap);
+/* Reads rows of the cache back as values (a * c in f32, rounded once to rows->dtype).  Rows of bad pages become zero. */
+int pcpb_op_kv_read(void* stream, const pcpb_kv_cache* cache, const pcpb_kv_rows* rows, int32_t* status, char* err, size_t err_cap);
+
+/* Attention of the nodes of drafted trees over the cache (bf16 in and out, f32 softmax).  Sequence b has the nodes
+ * [cu_nodes[b], cu_nodes[b + 1]) of q, k, v and out, at most max_nodes of them; parent[i] is a number within the sequence,
+ * smaller than the node's own, or -1 (parent NULL: a chain, node i under node i - 1).  Node i attends the first ctx_len[b]
+ * positions of the cache, its ancestors and itself:
+ *   out_i = sum_j w_ij v_j,  w_ij = softmax over j of scale * q_i . k_j;   query head h reads kv head h / (n_head / n_kv_head)
+ * The nodes' own keys and values come from k and v; they need not be in the cache (pcpb_op_kv_write adds the accepted ones
+ * afterwards).  A single token per sequence is a tree of one node.  null_self = 1: a node's own slot counts as a zero key
+ * and a zero value instead, the rule of the exported decode step (see pcpb_rollout above).
+ * The weights are rounded to bf16 before they meet the values (their sum is not); keys and values of 8-bit caches enter
+ * exactly, with their scales in f32 on the scores and the weights.  lse (optional) [n_rows][n_head] f32 receives the
+ * natural logarithm of each row's sum of exponentials.  Rows of out and lse behind cu_nodes[batch] are left as they are. */
+#define PCPB_TREE_MAX_NODES 256
+#define PCPB_TREE_MAX_BATCH 1024
+typedef struct pcpb_tree_attn {
+  const void *q, *k, *v;           /* bf16, element [row][head][i] at row * q_row + head * q_head + i */
+  void* out;
+  float* lse;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  const int32_t *cu_nodes, *parent, *ctx_len;
+  void* workspace;                 /* at least pcpb_op_tree_attention_workspace bytes, 16-byte aligned; contents do not matter */
+  size_t workspace_bytes;
+  int n_rows, n_head, max_nodes, null_self;
+  float scale;
+} pcpb_tree_attn;
+/* Bytes of workspace for a cache's geometry, n_head and max_nodes on a device (0 and *err when the arguments are refused). */
+size_t pcpb_op_tree_attention_workspace(int device_ordinal, const pcpb_kv_cache* cache, int n_head, int max_nodes, char* err, size_t err_cap);
+int pcpb_op_tree_attention(void* stream, const pcpb_kv_cache* cache, const pcpb_tree_attn* args, int32_t* status, char* err, size_t err_cap);
+
+/* Verification of drafted tokens.  logits row i belongs to node i (the target's prediction of what follows it); node 0 of
+ * a sequence is its last certain token, the others are drafts.  From node 0 on, p = softmax(logits / temperature); the
+ * children of the current node are tried in index order, child c with token t and its number u = u_accept[c] in [0, 1):
+ *   with draft_probs (row i: the distribution q that node i's children were drawn from): taken if u q_t D < max(p_t - a q_t, 0),
+ *     a = 0, D = 1 at first; after a refusal a += D, D = sum max(p - a q, 0)   (repeated rejection sampling)
+ *   without: taken if u D < p_t, D = 1 at first; after a refusal D -= p_t, p_t = 0   (drafts that were certain)
+ * (a refusal that would leave D <= 0 changes nothing).  A taken child's token is emitted and the walk goes on from it; when
+ * none is left, the last token is the first index whose running sum of the remaining weights passes u_sample[b] times their
+ * total.  So the emitted tokens are distributed as samples of p one by one.  temperature < 1e-6: children and the last token
+ * are compared with the first maximum of the logits (NaN never wins), as the engine's sampler does.  The walk also ends
+ * when max_out tokens are out.  Probabilities that a decision hangs on are formed in 64 bits.
+ *   tokens_out, path_out  [batch][max_out]: the emitted tokens (the rest 0) and the rows of the nodes they were emitted at
+ *                         (the rest -1): path_out, as pcpb_kv_rows.index, names the rows of k and v that are now certain
+ *   n_out                 [batch]: how many; 0 for a sequence without nodes
+ * A row whose logits have no finite maximum (or +inf) accepts no child and emits -1 (PCPB_OPS_NO_CHOICE). */
+typedef struct pcpb_verify {
+  const void* logits;              /* PCPB_BF16 or PCPB_F32, [n_rows][vocab] with row stride logits_row */
+  const float* draft_probs;        /* optional, f32, row stride draft_row */
+  long long logits_row, draft_row;
+  const int32_t *cu_nodes, *parent;
+  const int64_t* token;            /* [n_rows]; node 0's is not looked at */
+  const float *u_accept, *u_sample;
+  int64_t* tokens_out;
+  int32_t *path_out, *n_out;
+  double temperature;
+  int dtype, vocab, n_rows, batch, max_nodes, max_out;      /* max_nodes <= PCPB_TREE_MAX_NODES */
+} pcpb_verify;
+int pcpb_op_verify_drafts(void* stream, const pcpb_verify* args, int32_t* status, char* err, size_t err_cap);
 
 /* Kernel counters of this backend: launches enqueued since creation, by the library's own kernels. */
 long long pcpb_launch_count(const pcpb_backend* b);

@@ -48,7 +48,8 @@ EXPORTS = [
     "pcpb_init_master_elems", "pcpb_init_master", "pcpb_worker_write_state", "pcpb_worker_set_sampling",
     "pcpb_adjoint_status", "pcpb_rollout_num_params", "pcpb_rollout_create", "pcpb_rollout_destroy", "pcpb_rollout_last_error",
     "pcpb_rollout_load_weights", "pcpb_rollout_random_weights", "pcpb_rollout_generate", "pcpb_rollout_read_logits",
-    "pcpb_rollout_launch_count",
+    "pcpb_rollout_launch_count", "pcpb_op_kv_write", "pcpb_op_kv_read", "pcpb_op_tree_attention",
+    "pcpb_op_tree_attention_workspace", "pcpb_op_verify_drafts",
 ]
 ADJ_CLAMPED, ADJ_INTERNAL = 1, 2
 CHAR_VOCAB_MAX = 65

@@ -1,0 +1,589 @@
+// Attention of the nodes of drafted trees over a paged cache in bf16 or 8 bits.
+//
+//   out_i = sum_j w_ij v_j,  w_ij = exp2(z_ij - m_i) / l_i,  z_ij = scale log2(e) a_j (q_i . c_j),  m_i = max_j z_ij,  l_i = sum_j exp2(z_ij - m_i)
+//
+// in one pass over the keys with the running maximum and sum of a row (a_j: the key's scale, c_j its codes; values enter as
+// (w_ij b_j) d_j with b_j their scale).  Where a row's keys are split, the parts (O, m, l) are joined by
+//   m = max m_s,  l = sum exp2(m_s - m) l_s,  O = sum exp2(m_s - m) O_s.
+//
+// Work.  The rows of one item are those of a sequence's nodes and of the query heads of one kv head, node-major (row = node G + head),
+// in tiles of ROWS; its keys are the cached positions, then the nodes, in tiles of TILE.  All tiles of all items are laid end
+// to end, and block c of the grid takes the c-th equal share of them: ragged contexts balance, and one long context spreads
+// over the whole GPU.  Lengths are read on the device, so the grid does not depend on them.  An item that lies in one block is
+// finished there; the parts of the others go to the workspace (a block has at most two of them: the item it begins in and the
+// one it ends in) and k_tree_join adds them up in block order, so results do not depend on timing.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "decode_ops.h"
+
+namespace pcpb {
+namespace {
+
+constexpr int TILE = 128;            // keys of a scheduling step
+constexpr int MAX_NODES = PCPB_TREE_MAX_NODES, MAX_BATCH = PCPB_TREE_MAX_BATCH;
+constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+  pcpb_kv_cache c;
+  pcpb_tree_attn a;
+  int32_t* status;
+  int G;                             // query heads of a kv head
+  long long* plan;                   // workspace: [batch + 1] first tile of every sequence
+  float* part_ml;                    // [blocks][2][ROWS][2] maximum and sum
+  float* part_o;                     // [blocks][2][ROWS][HD]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four codes in a word -> two pairs of bf16 (exact: both code types have fewer significant bits than bf16).
+//   e4m3: sign and the seven other bits move to the bf16 fields of the same name; the exponent's bias then differs by
+//         127 - 7 = 120, which one product with 2^120 repairs, for subnormal codes as well.
+//   i8:   the code plus 128 in the low byte of 2^23's bit pattern is the float 2^23 + 128 + code.
+template <int CODE> __device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  if (CODE == PCPB_E4M3) {
+    const uint32_t t0 = __byte_perm(w, 0, 0x1404), t1 = __byte_perm(w, 0, 0x3424);
+    p01 = bmul2(((t0 >> 4) & 0x07F007F0u) | (t0 & 0x80008000u), 0x7B807B80u);
+    p23 = bmul2(((t1 >> 4) & 0x07F007F0u) | (t1 & 0x80008000u), 0x7B807B80u);
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    const float k = 8388608.f + 128.f;
+    p01 = pack2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650)) - k, __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7651)) - k);
+    p23 = pack2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7652)) - k, __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7653)) - k);
+  }
+}
+
+// Clipped lengths of sequence b.
+typedef SeqLen Seq;
+__device__ __forceinline__ Seq seq_of(const AttnArgs& A, int b) {
+  const Seq s = clip_seq(A.a.cu_nodes[b], A.a.cu_nodes[b + 1], A.a.ctx_len[b], A.a.n_rows, A.a.max_nodes, A.c.max_pages * A.c.page_tokens);
+  if (s.bad) op_note(A.status, PCPB_OPS_BAD_LENGTH);
+  return s;
+}
+__device__ __forceinline__ int tiles_of(int x) { return (x + TILE - 1) / TILE; }
+
+// plan[b] = first tile of sequence b, plan[batch] = all tiles; by the whole block, into shared memory.
+template <int ROWS> __device__ void make_plan(const AttnArgs& A, long long* plan) {
+  __shared__ long long wsum[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  long long base = 0;
+  for (int b0 = 0; b0 < A.c.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    long long x = 0;
+    if (b < A.c.batch) {
+      const Seq s = seq_of(A, b);
+      x = (long long)((s.n * A.G + ROWS - 1) / ROWS) * A.c.n_kv_head * (tiles_of(s.ctx) + tiles_of(s.n));
+    }
+    long long inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += y; }
+    if (lane == 31) wsum[w] = inc;
+    __syncthreads();
+    long long before = base, all = base;
+    for (int i = 0; i < nw; ++i) { if (i < w) before += wsum[i]; all += wsum[i]; }
+    if (b < A.c.batch) plan[b] = before + inc - x;
+    base = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) plan[A.c.batch] = base;
+  __syncthreads();
+}
+// The sequence tile t belongs to: plan[b] <= t < plan[b + 1]
+__device__ __forceinline__ int seq_at(const long long* plan, int batch, long long t) {
+  int lo = 0, hi = batch;                                       // plan[lo] <= t < plan[hi]
+  while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (plan[mid] <= t) lo = mid; else hi = mid; }
+  return lo;
+}
+
+// ---- the kernel for any number of rows: 16 a tile, mma.sync ---------------------------------------------------------
+// Eight warps share the 16 rows and split the keys in units of 16: no barrier until the item ends.  A lane's 16-byte pieces of keys
+// and values go straight from global memory into the fragments of mma.sync m16n8k16: which of the head_dim elements meet in one
+// k16 step does not matter as long as q is read with the same assignment, and which output columns a lane holds does not
+// matter as long as they are stored where they belong; so no element changes lanes.  Values are paired by position with byte
+// permutes.  The scores' fragment is the weights' operand of the second product as it stands.
+constexpr int RW = 16;               // rows of a tile
+constexpr int WARPS = 8;
+
+template <int HD, int CODE> struct Frag {
+  static constexpr int ES = CODE == PCPB_BF16 ? 2 : 1;
+  static constexpr int KB = HD * ES / 4 < 16 ? HD * ES / 4 : 16, KE = KB / ES, KC = HD / (4 * KE);   // bytes, elements of a lane's key piece; pieces a row
+  static constexpr int VB = HD * ES / 8 < 16 ? HD * ES / 8 : 16, VE = VB / ES, VC = HD / (8 * VE);
+};
+template <int BYTES> __device__ __forceinline__ void ld_bytes(const void* p, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES == 16) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+  else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+  else w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+
+template <int HD> struct RowState {
+  uint32_t q[HD / 16][4];
+  float o[HD / 8][4], m[2], l[2];
+};
+
+// q fragments of rows row0 .. row0 + 15 in the element order of Frag<HD, CODE>
+template <int HD, int CODE> __device__ __forceinline__ void load_q(const AttnArgs& A, const Seq& s, int kvh, int row0, RowState<HD>& R) {
+  typedef Frag<HD, CODE> F;
+  const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3, rows = s.n * A.G;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = row0 + g + 8 * half;
+    const bf16* p = (const bf16*)A.a.q + (long long)(s.n0 + r / A.G) * A.a.q_row + (long long)(kvh * A.G + r % A.G) * A.a.q_head;
+#pragma unroll
+    for (int st = 0; st < HD / 16; ++st) {
+      const int e = 4 * F::KE * (st / (F::KE / 4)) + F::KE * qd + 4 * (st % (F::KE / 4));
+      const uint2 v = r < rows ? *reinterpret_cast<const uint2*>(p + e) : make_uint2(0u, 0u);
+      R.q[st][half] = v.x; R.q[st][2 + half] = v.y;
+    }
+  }
+}
+
+// Output columns of accumulator tile t: element k of the fragment is row g + 8 (k >> 1), column col(t, 2 qd + (k & 1))
+template <int HD, int CODE> __device__ __forceinline__ int out_col(int t, int n) {
+  typedef Frag<HD, CODE> F;
+  return (t / F::VE) * 8 * F::VE + n * F::VE + t % F::VE;
+}
+
+// One unit of 16 keys.  krow / vrow: this lane's rows of keys (positions g, g + 8 of the unit) and values (2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd),
+// NULL where there is none; keep[half][i]: may row g + 8 half attend the score fragment's column i (positions 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd);
+// zero[half][i]: that slot counts as a zero key and value.
+// TREE: rows attend different keys of the unit.  A weight of 0 does not keep an infinity or a NaN of another branch's value out of the
+// matrix product, so a unit with such a value adds its products one by one, attended ones only.
+template <int HD, int CODE, bool TREE>
+__device__ __forceinline__ void unit(RowState<HD>& R, const uint8_t* const (&krow)[2], const uint8_t* const (&vrow)[4], const float (&ks)[4],
+                                     const float (&vs)[4], float zscale, const bool (&keep)[2][4], const bool (&zero)[2][4]) {
+  typedef Frag<HD, CODE> F;
+  const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
+  uint32_t kw[2][F::KC][F::KB / 4], vw[4][F::VC][F::VB / 4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int c = 0; c < F::KC; ++c) {
+#pragma unroll
+      for (int i = 0; i < F::KB / 4; ++i) kw[j][c][i] = 0u;
+      if (krow[j]) ld_bytes<F::KB>(krow[j] + (4 * F::KE * c + F::KE * qd) * F::ES, kw[j][c]);
+    }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int c = 0; c < F::VC; ++c) {
+#pragma unroll
+      for (int i = 0; i < F::VB / 4; ++i) vw[j][c][i] = 0u;
+      if (vrow[j]) ld_bytes<F::VB>(vrow[j] + (8 * F::VE * c + F::VE * g) * F::ES, vw[j][c]);
+    }
+  float s[2][4] = {};
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int st = 0; st < HD / 16; ++st) {
+      const int c = st / (F::KE / 4), sub = st % (F::KE / 4);
+      if (CODE == PCPB_BF16) {
+        mma16816(s[j], R.q[st], kw[j][c][(2 * sub) % (F::KB / 4)], kw[j][c][(2 * sub + 1) % (F::KB / 4)]);
+      } else {
+        uint32_t b0, b1;
+        widen4<CODE>(kw[j][c][sub % (F::KB / 4)], b0, b1);
+        mma16816(s[j], R.q[st], b0, b1);
+      }
+    }
+  // scores: s[j][2 half + i] is row g + 8 half, position 8 j + 2 qd + i
+  uint32_t p[4];
+  float corr[2], wt[2][4];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float z[4], mx = R.m[half];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[i] = s[i >> 1][2 * half + (i & 1)] * (zscale * ks[i]);
+      if (zero[half][i]) z[i] = 0.f;
+      if (!keep[half][i]) z[i] = -INFINITY;
+      mx = fmaxf(mx, z[i]);
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float ref = mx == -INFINITY ? 0.f : mx;               // a row that has seen nothing yet: every weight below is 0
+    corr[half] = ex2(R.m[half] - ref);
+    R.m[half] = mx;
+    float e[4], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = ex2(z[i] - ref);
+      sum += e[i];
+      e[i] = zero[half][i] ? 0.f : e[i] * vs[i];
+      if (TREE) wt[half][i] = bf16_round(e[i]);
+    }
+    R.l[half] = R.l[half] * corr[half] + sum;                   // this lane's share of the row's sum
+    p[half] = pack2(e[0], e[1]); p[2 + half] = pack2(e[2], e[3]);
+  }
+#pragma unroll
+  for (int t = 0; t < HD / 8; ++t) { R.o[t][0] *= corr[0]; R.o[t][1] *= corr[0]; R.o[t][2] *= corr[1]; R.o[t][3] *= corr[1]; }
+  if (TREE) {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < F::VC; ++c)
+#pragma unroll
+        for (int i = 0; i < F::VB / 4; ++i) odd |= (vw[j][c][i] & 0x7F80u) == 0x7F80u || (vw[j][c][i] & 0x7F800000u) == 0x7F800000u;
+    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {                           // key 8 (i >> 1) + 2 x + (i & 1): its weights are with lane x of the row's four
+          const int src = (lane & ~3) | x;
+          const bf16* v = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)vrow[i], src);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float w = __shfl_sync(0xffffffffu, wt[half][i], src);
+            const int on = __shfl_sync(0xffffffffu, (int)(keep[half][i] && !zero[half][i]), src);
+            if (!on) continue;
+#pragma unroll
+            for (int t = 0; t < HD / 8; ++t)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) R.o[t][2 * half + k] += w * to_f(v[out_col<HD, CODE>(t, 2 * qd + k)]);
+          }
+        }
+      return;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < F::VC; ++c)
+#pragma unroll
+    for (int i = 0; i < F::VB / 4; ++i) {
+      if (CODE == PCPB_BF16) {
+        mma16816(R.o[c * F::VE + 2 * i], p, __byte_perm(vw[0][c][i], vw[1][c][i], 0x5410), __byte_perm(vw[2][c][i], vw[3][c][i], 0x5410));
+        mma16816(R.o[c * F::VE + 2 * i + 1], p, __byte_perm(vw[0][c][i], vw[1][c][i], 0x7632), __byte_perm(vw[2][c][i], vw[3][c][i], 0x7632));
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a0, a1, b0, b1;
+          widen4<CODE>(__byte_perm(vw[0][c][i], vw[1][c][i], h ? 0x7362 : 0x5140), a0, a1);
+          widen4<CODE>(__byte_perm(vw[2][c][i], vw[3][c][i], h ? 0x7362 : 0x5140), b0, b1);
+          mma16816(R.o[c * F::VE + 4 * i + 2 * h], p, a0, b0);
+          mma16816(R.o[c * F::VE + 4 * i + 2 * h + 1], p, a1, b1);
+        }
+      }
+    }
+}
+// Ancestors-or-self of the nodes of a tile's rows, 256 bits a row, in shared memory
+__device__ void make_ancestors(const AttnArgs& A, const Seq& s, int row0, int rows_tile, int16_t* par, uint32_t (*anc)[MAX_NODES / 32]) {
+  for (int i = threadIdx.x; i < s.n; i += blockDim.x) {
+    int bad = 0;
+    par[i] = (int16_t)clip_parent(A.a.parent ? A.a.parent[s.n0 + i] : i - 1, i, &bad);
+    if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < rows_tile; r += blockDim.x) {
+    uint32_t w[MAX_NODES / 32] = {};
+    int i = (row0 + r) / A.G;
+    if (i < s.n)
+      while (i >= 0) {                                          // parents come before their children: at most n steps
+#pragma unroll
+        for (int k = 0; k < MAX_NODES / 32; ++k) w[k] |= (i >> 5) == k ? 1u << (i & 31) : 0u;
+        i = par[i];
+      }
+#pragma unroll
+    for (int k = 0; k < MAX_NODES / 32; ++k) anc[r][k] = w[k];
+  }
+  __syncthreads();
+}
+
+template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_tree_rows(const __grid_constant__ AttnArgs A) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  long long* plan = reinterpret_cast<long long*>(smem);                       // [batch + 1]
+  float* mo = reinterpret_cast<float*>(smem + ((A.c.batch + 1) * 8 + 15) / 16 * 16);   // [WARPS][RW][HD]
+  __shared__ float mml[WARPS][RW][2];
+  __shared__ int16_t par[MAX_NODES];
+  __shared__ uint32_t anc[RW][MAX_NODES / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
+  make_plan<RW>(A, plan);
+  const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
+  if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
+  const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
+  const float zscale = A.a.scale * LOG2E;
+  const bool none[2][4] = {};
+  for (long long w = w0; w < w1;) {
+    const int b = seq_at(plan, A.c.batch, w);
+    const Seq s = seq_of(A, b);
+    const int ct = tiles_of(s.ctx), T = ct + tiles_of(s.n), RT = (s.n * A.G + RW - 1) / RW;
+    const long long item = (w - plan[b]) / T;
+    const int t0 = (int)((w - plan[b]) % T), t1 = (int)min((long long)T, t0 + (w1 - w));
+    const int kvh = (int)(item / RT), row0 = (int)(item % RT) * RW, rows = s.n * A.G;
+    RowState<HD> R;
+#pragma unroll
+    for (int t = 0; t < HD / 8; ++t) R.o[t][0] = R.o[t][1] = R.o[t][2] = R.o[t][3] = 0.f;
+    R.m[0] = R.m[1] = -INFINITY; R.l[0] = R.l[1] = 0.f;
+    // cached keys [t0 TILE, t1 TILE)
+    if (t0 < ct) {
+      load_q<HD, CODE>(A, s, kvh, row0, R);
+      const int end = min(s.ctx, t1 * TILE);
+      constexpr int ES = Frag<HD, CODE>::ES;
+      for (int u = t0 * TILE + warp * 16; u < end; u += WARPS * 16) {
+        const int pos = u + (lane & 15);                        // lanes 0 .. 15 find the rows of the unit's positions
+        const int page = pos < end ? page_of(A.c, b, pos / A.c.page_tokens) : -1;
+        if (pos < end && page < 0) op_note(A.status, PCPB_OPS_BAD_PAGE);
+        const int in_page = pos % A.c.page_tokens;
+        const long long off = page < 0 ? -1 : page_row(page, A.c.page_stride, kvh, A.c.page_tokens, in_page, HD) * ES;
+        const long long soff = page < 0 ? -1 : page_row(page, A.c.scale_stride, kvh, A.c.page_tokens, in_page, 1);
+        const uint8_t *krow[2], *vrow[4];
+        float ks[4], vs[4];
+        bool keep[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const long long o = __shfl_sync(0xffffffffu, off, 8 * j + g);
+          krow[j] = o < 0 ? nullptr : (const uint8_t*)A.c.k + o;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = 8 * (i >> 1) + 2 * qd + (i & 1);
+          const long long o = __shfl_sync(0xffffffffu, off, at), so = __shfl_sync(0xffffffffu, soff, at);
+          vrow[i] = o < 0 ? nullptr : (const uint8_t*)A.c.v + o;
+          keep[0][i] = keep[1][i] = o >= 0;
+          ks[i] = vs[i] = 1.f;
+          if (CODE != PCPB_BF16 && o >= 0) { ks[i] = A.c.k_scale[so]; vs[i] = A.c.v_scale[so]; }
+        }
+        unit<HD, CODE, false>(R, krow, vrow, ks, vs, zscale, keep, none);
+      }
+    }
+    // the nodes' own keys
+    if (t1 > ct) {
+      make_ancestors(A, s, row0, RW, par, anc);
+      load_q<HD, PCPB_BF16>(A, s, kvh, row0, R);
+      RowState<HD> N;                                           // 8-bit caches: the nodes' keys are bf16, with their own order of q and columns
+      const int lo = max(t0 - ct, 0) * TILE, end = min(s.n, (t1 - ct) * TILE);
+#pragma unroll
+      for (int t = 0; t < HD / 8; ++t) N.o[t][0] = N.o[t][1] = N.o[t][2] = N.o[t][3] = 0.f;
+#pragma unroll
+      for (int t = 0; t < HD / 16; ++t) for (int i = 0; i < 4; ++i) N.q[t][i] = R.q[t][i];
+      N.m[0] = N.m[1] = -INFINITY; N.l[0] = N.l[1] = 0.f;
+      const float one[4] = {1.f, 1.f, 1.f, 1.f};
+      for (int u = lo + warp * 16; u < end; u += WARPS * 16) {
+        const uint8_t *krow[2], *vrow[4];
+        bool keep[2][4], zero[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = u + 8 * j + g;
+          krow[j] = i < end ? (const uint8_t*)((const bf16*)A.a.k + (long long)(s.n0 + i) * A.a.k_row + (long long)kvh * A.a.k_head) : nullptr;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = u + 8 * (j >> 1) + 2 * qd + (j & 1);
+          vrow[j] = i < end ? (const uint8_t*)((const bf16*)A.a.v + (long long)(s.n0 + i) * A.a.v_row + (long long)kvh * A.a.v_head) : nullptr;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = g + 8 * half;
+            keep[half][j] = i < end && ((anc[r][(i >> 5) & 7] >> (i & 31)) & 1u);
+            zero[half][j] = A.a.null_self && i == (row0 + r) / A.G;
+          }
+        }
+        unit<HD, PCPB_BF16, true>(N, krow, vrow, one, one, zscale, keep, zero);
+      }
+      // join both parts: through shared memory, since the columns of a lane differ between the two
+      if (CODE != PCPB_BF16) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float m = fmaxf(R.m[half], N.m[half]), ref = m == -INFINITY ? 0.f : m;
+          const float cr = ex2(R.m[half] - ref), cn = ex2(N.m[half] - ref);
+          R.l[half] = R.l[half] * cr + N.l[half] * cn; R.m[half] = m;
+          float* row = mo + ((size_t)warp * RW + g + 8 * half) * HD;
+#pragma unroll
+          for (int t = 0; t < HD / 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              row[out_col<HD, PCPB_BF16>(t, 2 * qd + i)] = N.o[t][2 * half + i] * cn;
+              R.o[t][2 * half + i] *= cr;
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int t = 0; t < HD / 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              R.o[t][2 * half + i] += mo[((size_t)warp * RW + g + 8 * half) * HD + out_col<HD, CODE>(t, 2 * qd + i)];
+        __syncwarp();
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float m = fmaxf(R.m[half], N.m[half]), ref = m == -INFINITY ? 0.f : m;
+          const float cr = ex2(R.m[half] - ref), cn = ex2(N.m[half] - ref);
+          R.l[half] = R.l[half] * cr + N.l[half] * cn; R.m[half] = m;
+#pragma unroll
+          for (int t = 0; t < HD / 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) R.o[t][2 * half + i] = R.o[t][2 * half + i] * cr + N.o[t][2 * half + i] * cn;
+        }
+      }
+    }
+    // the eight warps' parts -> the tile's rows
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float l = R.l[half];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (qd == 0) { mml[warp][g + 8 * half][0] = R.m[half]; mml[warp][g + 8 * half][1] = l; }
+#pragma unroll
+      for (int t = 0; t < HD / 8; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) mo[((size_t)warp * RW + g + 8 * half) * HD + out_col<HD, CODE>(t, 2 * qd + i)] = R.o[t][2 * half + i];
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == T;
+    const size_t slot = (size_t)blockIdx.x * 2 + (w == w0 ? 0 : 1);
+    for (int i = threadIdx.x; i < RW * (HD / 4); i += blockDim.x) {
+      const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+      if (row0 + r >= rows) continue;
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) m = fmaxf(m, mml[k][r][0]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l = 0.f, o[4] = {};
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) {
+        const float f = ex2(mml[k][r][0] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(mo + ((size_t)k * RW + r) * HD + c);
+        l += f * mml[k][r][1];
+        o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
+      }
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int node = (row0 + r) / A.G, h = kvh * A.G + (row0 + r) % A.G;
+        bf16* dst = (bf16*)A.a.out + (long long)(s.n0 + node) * A.a.out_row + (long long)h * A.a.out_head + c;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+        if (A.a.lse && c == 0) A.a.lse[(size_t)(s.n0 + node) * A.a.n_head + h] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
+      } else {
+        *reinterpret_cast<float4*>(A.part_o + (slot * RW + r) * HD + c) = make_float4(o[0], o[1], o[2], o[3]);
+        if (c == 0) { A.part_ml[(slot * RW + r) * 2] = m; A.part_ml[(slot * RW + r) * 2 + 1] = l; }
+      }
+    }
+    __syncthreads();
+    w += t1 - t0;
+  }
+}
+
+// Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles), one thread per four columns of a row.
+template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ AttnArgs A, int blocks) {
+  const int b = blockIdx.x;
+  const Seq s = seq_of(A, b);
+  const int rows = s.n * A.G, RT = (rows + ROWS - 1) / ROWS, T = tiles_of(s.ctx) + tiles_of(s.n);
+  const int item = blockIdx.y;
+  if (item >= RT * A.c.n_kv_head) return;
+  const Parts P = parts_of(A.plan[b] + (long long)item * T, T, tile_share(A.plan[A.c.batch], blocks));
+  if (P.c0 == P.c1) return;
+  const int kvh = item / RT, row0 = item % RT * ROWS;
+  for (int i = threadIdx.x; i < ROWS * (HD / 4); i += blockDim.x) {
+    const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+    if (row0 + r >= rows) continue;
+    float m = -INFINITY;
+    for (int k = P.c0; k <= P.c1; ++k) m = fmaxf(m, A.part_ml[((size_t)part_slot(P, k) * ROWS + r) * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[4] = {};
+    for (int k = P.c0; k <= P.c1; ++k) {
+      const size_t at = (size_t)part_slot(P, k) * ROWS + r;
+      const float f = ex2(A.part_ml[at * 2] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(A.part_o + at * HD + c);
+      l += f * A.part_ml[at * 2 + 1];
+      o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int node = (row0 + r) / A.G, h = kvh * A.G + (row0 + r) % A.G;
+    bf16* dst = (bf16*)A.a.out + (long long)(s.n0 + node) * A.a.out_row + (long long)h * A.a.out_head + c;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+    if (A.a.lse && c == 0) A.a.lse[(size_t)(s.n0 + node) * A.a.n_head + h] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+int sm_count(int dev) {
+  int n = 0;
+  return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+}
+struct Layout { size_t plan, ml, o, bytes; };
+Layout layout(const pcpb_kv_cache& c, int blocks, int rows_tile) {
+  Layout L;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  L.plan = 0;
+  L.ml = up((size_t)(c.batch + 1) * 8);
+  L.o = L.ml + up((size_t)blocks * 2 * rows_tile * 2 * 4);
+  L.bytes = L.o + up((size_t)blocks * 2 * rows_tile * c.head_dim * 4);
+  return L;
+}
+int check_heads(const pcpb_kv_cache& c, int n_head, int max_nodes, char* err, size_t cap) {
+  if (n_head < 1 || n_head % c.n_kv_head) return op_fail(err, cap, PCPB_E_INVALID, "n_head must be a multiple of n_kv_head");
+  if (max_nodes < 1) return op_fail(err, cap, PCPB_E_INVALID, "max_nodes must be positive");
+  if (max_nodes > MAX_NODES) return op_fail(err, cap, PCPB_E_TOO_LARGE, "at most %d nodes a sequence", MAX_NODES);
+  if (c.batch > MAX_BATCH) return op_fail(err, cap, PCPB_E_TOO_LARGE, "at most %d sequences a call", MAX_BATCH);
+  const long long items = (long long)c.n_kv_head * ((max_nodes * (long long)(n_head / c.n_kv_head) + RW - 1) / RW);
+  if (items > 65535) return op_fail(err, cap, PCPB_E_TOO_LARGE, "too many query heads");
+  return PCPB_OK;
+}
+
+template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnArgs& A, int blocks) {
+  const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)WARPS * RW * HD * 4;
+  cudaError_t e = cudaFuncSetAttribute(k_tree_rows<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  k_tree_rows<HD, CODE><<<blocks, WARPS * 32, smem, st>>>(A);
+  const int items = A.c.n_kv_head * ((A.a.max_nodes * A.G + RW - 1) / RW);
+  k_tree_join<HD, RW><<<dim3(A.c.batch, items), 256, 0, st>>>(A, blocks);
+  return cudaGetLastError();
+}
+template <int HD> cudaError_t launch_code(cudaStream_t st, const AttnArgs& A, int blocks) {
+  if (A.c.dtype == PCPB_BF16) return launch_rows<HD, PCPB_BF16>(st, A, blocks);
+  if (A.c.dtype == PCPB_I8) return launch_rows<HD, PCPB_I8>(st, A, blocks);
+  return launch_rows<HD, PCPB_E4M3>(st, A, blocks);
+}
+
+}  // namespace
+}  // namespace pcpb
+
+using namespace pcpb;
+
+extern "C" size_t pcpb_op_tree_attention_workspace(int device, const pcpb_kv_cache* cache, int n_head, int max_nodes, char* err, size_t cap) {
+  if (err && cap) err[0] = 0;
+  pcpb_kv_cache c;
+  if (check_cache(cache, &c, err, cap) || check_heads(c, n_head, max_nodes, err, cap)) return 0;
+  return layout(c, sm_count(device), RW).bytes;
+}
+
+extern "C" int pcpb_op_tree_attention(void* stream, const pcpb_kv_cache* cache, const pcpb_tree_attn* args, int32_t* status, char* err, size_t cap) {
+  if (err && cap) err[0] = 0;
+  AttnArgs A;
+  int rc = check_cache(cache, &A.c, err, cap);
+  if (rc) return rc;
+  if (!args) return op_fail(err, cap, PCPB_E_INVALID, "null arguments");
+  A.a = *args; A.status = status;
+  const pcpb_tree_attn& a = A.a;
+  if ((rc = check_heads(A.c, a.n_head, a.max_nodes, err, cap))) return rc;
+  A.G = a.n_head / A.c.n_kv_head;
+  if (a.n_rows < 0) return op_fail(err, cap, PCPB_E_INVALID, "negative row count");
+  if (a.n_rows == 0) return PCPB_OK;
+  if (!a.q || !a.k || !a.v || !a.out || !a.cu_nodes || !a.ctx_len || !a.workspace) return op_fail(err, cap, PCPB_E_INVALID, "null argument");
+  if (!rows_aligned(a.q, a.q_row, a.q_head, 2) || !rows_aligned(a.k, a.k_row, a.k_head, 2) || !rows_aligned(a.v, a.v_row, a.v_head, 2) ||
+      !rows_aligned(a.out, a.out_row, a.out_head, 2))
+    return op_fail(err, cap, PCPB_E_INVALID, "rows of q, k, v and out must start on 16-byte boundaries");
+  if (!aligned16(a.workspace)) return op_fail(err, cap, PCPB_E_INVALID, "the workspace must start on a 16-byte boundary");
+  OpDevice d(err, cap);
+  on_cache(d, A.c);
+  d.on(a.q, "q"); d.on(a.k, "k"); d.on(a.v, "v"); d.on(a.out, "out"); d.on(a.lse, "lse"); d.on(a.cu_nodes, "cu_nodes"); d.on(a.parent, "parent");
+  d.on(a.ctx_len, "ctx_len"); d.on(a.workspace, "workspace"); d.on(status, "status");
+  if (d.enter()) return d.rc;
+  const int blocks = sm_count(d.dev);
+  const Layout L = layout(A.c, blocks, RW);
+  if (a.workspace_bytes < L.bytes)
+    return op_fail(err, cap, PCPB_E_INVALID, "workspace of %zu bytes, %zu are needed (pcpb_op_tree_attention_workspace)", a.workspace_bytes, L.bytes);
+  uint8_t* ws = (uint8_t*)a.workspace;
+  A.plan = (long long*)(ws + L.plan); A.part_ml = (float*)(ws + L.ml); A.part_o = (float*)(ws + L.o);
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (A.c.head_dim == 128) e = launch_code<128>(st, A, blocks);
+  else if (A.c.head_dim == 64) e = launch_code<64>(st, A, blocks);
+  else e = launch_code<32>(st, A, blocks);
+  return d.done(e);
+}

@@ -4,8 +4,16 @@
 //   after a refusal a += D, D = sum_i max(p_i - a q_i, 0): with r_0 = p and r_{k+1} = max(r_k - q, 0) / Z_k one finds by induction
 //   r_k = max(p - a_k q, 0) / D_k with a_{k+1} = a_k + D_k, so the k-th residual needs p, q and two numbers.
 //
-// Only the rows of the nodes on the accepted path are read.  Sums are 64-bit: a decision that hangs on the last bits of a probability then
-// comes out as the definition's.
+// Bound: latency.  Only the rows of the nodes on the accepted path have to be read, one after the other, so a step's time is that of one row
+// (304 KB at 151936 words): a cluster of up to 16 blocks takes a sequence, every warp a contiguous segment of the row.  Per step the warps'
+// maxima and sums go to all blocks of the cluster through distributed shared memory, and after ONE cluster barrier every thread
+// makes the same decision from the same numbers; buffers alternate, so the next exchange needs no second barrier.
+//
+// Precision.  Sums of a step are f32.  S is off (relative) by at most 2^-22 of exp2, three roundings of its argument, whose weighted mean
+// is at most log2 V (3 ln 2 log2(V) 2^-24 = 2.1e-6), as much again and 2^-22 for each of the dozen joins of parts, and the
+// additions of a thread's V / 4096 terms: below 8e-6 + V / 4096 2^-24.  A decision within twice that is made again with a 64-bit S; the
+// residuals and the running sum for the last token are 64-bit throughout.  So the result is that of 64-bit arithmetic.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -14,151 +22,403 @@
 namespace pcpb {
 namespace {
 
-constexpr int VT = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int VT = 256, VW = VT / 32;              // threads and warps of a block
+constexpr int MAX_CL = 16;                         // blocks of a cluster
+constexpr int MAX_N = PCPB_TREE_MAX_NODES;
+constexpr int AHEAD_N = 64;                        // most nodes whose rows are all read ahead of the walk
+constexpr double AHEAD_BYTES = 32e6;
 
 struct VerifyArgs {
   pcpb_verify v;
   int32_t* status;
+  int ahead;                                       // read every node's row first, walk afterwards
 };
 
-__device__ __forceinline__ double block_sum_d(double x, double* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  double s = 0.0;
-  for (int i = 0; i < VT / 32; ++i) s += red[i];
-  return s;
+struct Stat { float m, s; int at; };               // maximum, sum of exp2((z - m) c), first index of the maximum
+__device__ __forceinline__ float fast_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool GREEDY> __device__ __forceinline__ void stat_join(Stat& a, const Stat& b, float c) {
+  if (GREEDY) {
+    if (b.m > a.m || (b.m == a.m && b.at < a.at)) a = b;
+  } else {
+    const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+    a.s = a.s * fast_ex2((a.m - ref) * c) + b.s * fast_ex2((b.m - ref) * c);
+    a.m = m;
+  }
 }
 
-// Weight of index i in the distribution that is left: row z, draft row q, a, and the refused tokens
-template <typename T> struct Row {
+// A row of logits as 16-byte pieces: piece j holds the elements [j E - shift, (j + 1) E - shift) of the row; the first and the last may be short.
+template <typename T> struct Pieces {
+  static constexpr int E = 16 / sizeof(T);
   const T* z;
-  const float* q;
-  double zmax, invT, invS, a;
-  __device__ __forceinline__ double p(int i) const {
-    const double x = (double)to_f<T>(z[i]);
-    return x == x ? exp((x - zmax) * invT) * invS : 0.0;
+  int V, shift, n;
+  __device__ __forceinline__ Pieces(const T* row, int vocab) : z(row), V(vocab) {
+    shift = (int)(((uintptr_t)row & 15) / sizeof(T));
+    n = (V + shift + E - 1) / E;
   }
-  __device__ __forceinline__ double w(int i) const {
-    if (!q) return p(i);
-    const double r = p(i) - a * (double)q[i];
-    return r > 0.0 ? r : 0.0;
+  __device__ __forceinline__ int first(int j) const { return j * E - shift; }
+  // values of piece j, -inf where there is no element or a NaN
+  __device__ __forceinline__ void load(int j, float (&f)[E]) const {
+    const int i0 = first(j);
+    if (j < n && i0 >= 0 && i0 + E <= V) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(z + i0));
+      const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 2) { f[(2 * i) % E] = bf_lo(r[i]); f[(2 * i + 1) % E] = bf_hi(r[i]); }
+        else f[i] = __uint_as_float(r[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = j < n && i0 + i >= 0 && i0 + i < V ? to_f<T>(z[i0 + i]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = fmaxf(f[i], -INFINITY);
   }
 };
 
-template <typename T> __global__ void __launch_bounds__(VT) k_verify(const __grid_constant__ VerifyArgs A) {
-  __shared__ double red[VT / 32];
-  __shared__ float bv[VT / 32];
-  __shared__ int bi[VT / 32];
-  __shared__ int16_t par[PCPB_TREE_MAX_NODES];
-  __shared__ int refused[PCPB_TREE_MAX_NODES];
-  __shared__ int pick;
+// Maximum and sum of pieces [j0, j1) of a row, by a warp (a lane's own share; joined by the caller)
+template <typename T, bool GREEDY> __device__ __forceinline__ Stat scan(const Pieces<T>& P, int j0, int j1, float c) {
+  constexpr int E = Pieces<T>::E, U = 4;                         // pieces in flight per lane
+  Stat a{-INFINITY, 0.f, 0x7fffffff};
+  for (int j = j0 + (threadIdx.x & 31); j < j1; j += 32 * U) {
+    float f[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j + 32 * u < j1) P.load(j + 32 * u, f[u]);
+      else
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[u][i] = -INFINITY;
+    }
+    float m = a.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (GREEDY && f[u][i] > m) a.at = P.first(j + 32 * u) + i;       // ascending: the first index of the maximum
+        m = fmaxf(m, f[u][i]);
+      }
+    if (!GREEDY) {
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = a.s * fast_ex2((a.m - ref) * c);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += fast_ex2((f[u][i] - ref) * c);
+      a.s = s;
+    }
+    a.m = m;
+  }
+  return a;
+}
+template <bool GREEDY> __device__ __forceinline__ Stat warp_join(Stat a, float c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o); b.s = __shfl_xor_sync(0xffffffffu, a.s, o); b.at = __shfl_xor_sync(0xffffffffu, a.at, o);
+    stat_join<GREEDY>(a, b, c);
+  }
+  // lane 0's: the lanes' sums may differ in the last bit, and every thread of the cluster has to decide from the same numbers
+  a.m = __shfl_sync(0xffffffffu, a.m, 0); a.s = __shfl_sync(0xffffffffu, a.s, 0); a.at = __shfl_sync(0xffffffffu, a.at, 0);
+  return a;
+}
+
+struct Shared {
+  Stat stat[2][MAX_CL * VW];                       // one exchange: an entry from every warp of the cluster
+  double sum[2][MAX_CL * VW];
+  Stat ahead[AHEAD_N][MAX_CL];                     // AHEAD: an entry of every block for every row
+  Stat mine[AHEAD_N][VW];
+  long long token[MAX_N];
+  float u[MAX_N];
+  int16_t par[MAX_N];
+  int16_t kid[MAX_N];                              // the current node's children in index order, and what a decision needs of them
+  float kz[MAX_N], kq[MAX_N];
+  uint8_t gone[MAX_N];                             // the child's token has no weight left
+  int nkid;
+};
+
+// What is left of a row's distribution: weights max(e_i - aS q_i, 0) with e_i = exp((z_i - max) / T), the refused tokens' weights 0.
+template <typename T> struct Left {
+  Pieces<T> P;
+  const float* q;
+  double zmax, invT, aS;
+  int nref;                                        // refused tokens: those of the first nref children with gone[] set
+  __device__ __forceinline__ double weight(float z, int i, const Shared& sh) const {
+    if (z == -INFINITY) return 0.0;
+    double w = exp(((double)z - zmax) * invT);
+    if (q) { w -= aS * (double)__ldg(q + i); return w > 0.0 ? w : 0.0; }
+    return w;
+  }
+  // weights of piece j
+  __device__ __forceinline__ void weights(int j, const Shared& sh, double (&w)[Pieces<T>::E]) const {
+    constexpr int E = Pieces<T>::E;
+    float f[E];
+    P.load(j, f);
+    const int i0 = P.first(j);
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = weight(f[i], i0 + i, sh);
+    for (int k = 0; k < nref; ++k) {
+      const long long d = sh.token[sh.kid[k]] - i0;
+      if (sh.gone[k] && d >= 0 && d < E)
+#pragma unroll
+        for (int i = 0; i < E; ++i) if (i == (int)d) w[i] = 0.0;
+    }
+  }
+};
+
+template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verify(const __grid_constant__ VerifyArgs A) {
+  __shared__ Shared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  cl.barrier_arrive();                                          // waited for before the first write into another block
   const pcpb_verify& v = A.v;
-  const int b = blockIdx.x, tid = threadIdx.x, V = v.vocab;
+  const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank(), b = (int)blockIdx.x / CL;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = v.vocab;
   const SeqLen s = clip_seq(v.cu_nodes[b], v.cu_nodes[b + 1], 0, v.n_rows, v.max_nodes, 0);
   if (s.bad) op_note(A.status, PCPB_OPS_BAD_LENGTH);
   const int lo = s.n0, n = s.n;
+  const bool writer = rank == 0 && tid == 0;
+  const float c = GREEDY ? 1.f : (float)(1.4426950408889634 / v.temperature);
   for (int i = tid; i < n; i += VT) {
     int bad = 0;
-    par[i] = (int16_t)clip_parent(v.parent ? v.parent[lo + i] : i - 1, i, &bad);
+    sh.par[i] = (int16_t)clip_parent(v.parent ? v.parent[lo + i] : i - 1, i, &bad);
     if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
+    sh.token[i] = v.token[lo + i];
+    sh.u[i] = GREEDY ? 0.f : v.u_accept[lo + i];
   }
-  for (int i = tid; i < v.max_out; i += VT) { v.tokens_out[(size_t)b * v.max_out + i] = 0; v.path_out[(size_t)b * v.max_out + i] = -1; }
+  if (rank == 0)
+    for (int i = tid; i < v.max_out; i += VT) { v.tokens_out[(size_t)b * v.max_out + i] = 0; v.path_out[(size_t)b * v.max_out + i] = -1; }
+  // the warp's share of a row's n pieces
+  auto share = [&](int pieces, int* j0, int* j1) {
+    const int parts = CL * VW, per = (pieces + parts - 1) / parts, w = rank * VW + warp;
+    *j0 = min(pieces, w * per); *j1 = min(pieces, *j0 + per);
+  };
+  const double slack = 1.6e-5 + V * (1.0 / 4096 / 8388608);
+  int turn = 0;                                                 // buffer of the next exchange
+  // an f64 value of every warp -> the sum over all, in warp order; the values stay in sh.sum[*which]
+  auto exchange = [&](double x, int* which) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane < CL) *cl.map_shared_rank(&sh.sum[turn][rank * VW + warp], lane) = x;
+    cl.sync();
+    double t = 0.0;
+    for (int i = lane; i < CL * VW; i += 32) t += sh.sum[turn][i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    *which = turn;
+    turn ^= 1;
+    return t;
+  };
+  const bool ahead = A.ahead && n <= AHEAD_N;
   __syncthreads();
-  const bool greedy = v.temperature < 1e-6;
+  cl.barrier_wait();
+  if (ahead && n > 0) {
+    for (int i = 0; i < n; ++i) {
+      const Pieces<T> P((const T*)v.logits + (size_t)(lo + i) * v.logits_row, V);
+      int j0, j1;
+      share(P.n, &j0, &j1);
+      const Stat a = warp_join<GREEDY>(scan<T, GREEDY>(P, j0, j1, c), c);
+      if (lane == 0) sh.mine[i][warp] = a;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += VT) {
+      Stat a = sh.mine[i][0];
+      for (int w = 1; w < VW; ++w) stat_join<GREEDY>(a, sh.mine[i][w], c);
+      for (int r = 0; r < CL; ++r) *cl.map_shared_rank(&sh.ahead[i][rank], r) = a;
+    }
+    cl.sync();
+  }
   int node = 0, level = 0;
   while (n > 0 && level < v.max_out) {
-    Row<T> row;
-    row.z = (const T*)v.logits + (size_t)(lo + node) * v.logits_row;
-    row.q = v.draft_probs && !greedy ? v.draft_probs + (size_t)(lo + node) * v.draft_row : nullptr;
-    // first maximum
-    float best = -INFINITY;
-    int at = 0x7fffffff;
-    for (int i = tid; i < V; i += VT) { const float x = to_f<T>(row.z[i]); if (x > best) { best = x; at = i; } }
+    const T* zrow = (const T*)v.logits + (size_t)(lo + node) * v.logits_row;
+    const float* qrow = !GREEDY && v.draft_probs ? v.draft_probs + (size_t)(lo + node) * v.draft_row : nullptr;
+    const Pieces<T> P(zrow, V);
+    int j0, j1;
+    share(P.n, &j0, &j1);
+    if (warp == 0) {                                            // children, while the other warps read the row
+      int cnt = 0;
+      if (level + 1 < v.max_out)
+        for (int base = node + 1; base < n; base += 32) {
+          const int i = base + lane;
+          const bool is = i < n && sh.par[i] == node;
+          const bool in = is && sh.token[i] >= 0 && sh.token[i] < V;
+          if (is && !in) op_note(A.status, PCPB_OPS_NO_CHOICE);
+          const uint32_t bal = __ballot_sync(0xffffffffu, in);
+          if (in) {
+            const int k = cnt + __popc(bal & ((1u << lane) - 1));
+            sh.kid[k] = (int16_t)i;
+            sh.gone[k] = 0;
+            if (!GREEDY) { sh.kz[k] = to_f<T>(zrow[sh.token[i]]); sh.kq[k] = qrow ? qrow[sh.token[i]] : 1.f; }
+          }
+          cnt += __popc(bal);
+        }
+      if (lane == 0) sh.nkid = cnt;
+    }
+    Stat st;
+    if (ahead) {
+      __syncthreads();
+      st = Stat{-INFINITY, 0.f, 0x7fffffff};
+      if (lane < CL) st = sh.ahead[node][lane];
+      st = warp_join<GREEDY>(st, c);
+    } else {
+      const Stat a = warp_join<GREEDY>(scan<T, GREEDY>(P, j0, j1, c), c);
+      if (lane < CL) *cl.map_shared_rank(&sh.stat[turn][rank * VW + warp], lane) = a;
+      cl.sync();
+      st = Stat{-INFINITY, 0.f, 0x7fffffff};
+      for (int i = lane; i < CL * VW; i += 32) stat_join<GREEDY>(st, sh.stat[turn][i], c);
+      st = warp_join<GREEDY>(st, c);
+      turn ^= 1;
+    }
+    const bool choice = isfinite(st.m);
+    if (!choice && writer) op_note(A.status, PCPB_OPS_NO_CHOICE);
+    int taken = -1;
+    const int nkid = choice ? sh.nkid : 0;
+    if (GREEDY) {
+      for (int k = lane; k < nkid + lane; k += 32) {            // the first child with the winning token
+        const uint32_t hit = __ballot_sync(0xffffffffu, k < nkid && sh.token[sh.kid[k < nkid ? k : 0]] == st.at);
+        if (hit) { taken = sh.kid[k - lane + __ffs(hit) - 1]; break; }
+      }
+    }
+    Left<T> left{P, qrow, (double)st.m, GREEDY ? 1.0 : 1.0 / v.temperature, 0.0, 0};
+    double S = (double)st.s, a = 0.0, a0 = 0.0, D = 1.0;
+    bool sure = false;                                          // S is a 64-bit sum
+    int which;
+    auto sum_left = [&]() {                                     // sum of the weights that are left
+      double x = 0.0;
+      left.aS = a * S;
+      for (int j = j0 + lane; j < j1; j += 32) {
+        double w[Pieces<T>::E];
+        left.weights(j, sh, w);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-      if (ov > best || (ov == best && oi < at)) { best = ov; at = oi; }
-    }
-    __syncthreads();
-    if ((tid & 31) == 0) { bv[tid >> 5] = best; bi[tid >> 5] = at; }
-    __syncthreads();
-    best = bv[0]; at = bi[0];
-    for (int k = 1; k < VT / 32; ++k) if (bv[k] > best || (bv[k] == best && bi[k] < at)) { best = bv[k]; at = bi[k]; }
-    const bool choice = isfinite(best);
-    int taken = -1, nref = 0;
-    long long last = choice ? at : -1;
-    if (!choice && tid == 0) op_note(A.status, PCPB_OPS_NO_CHOICE);
-    if (choice && !greedy) {
-      row.zmax = best; row.invT = 1.0 / v.temperature; row.a = 0.0; row.invS = 1.0;
-      double s = 0.0;
-      for (int i = tid; i < V; i += VT) s += row.p(i);
-      row.invS = 1.0 / block_sum_d(s, red);
-    }
-    double D = 1.0;
-    if (choice && level + 1 < v.max_out)
-      for (int c = node + 1; c < n && taken < 0; ++c) {
-        if (par[c] != node) continue;
-        const long long t = v.token[lo + c];
-        if (t < 0 || t >= V) { if (tid == 0) op_note(A.status, PCPB_OPS_NO_CHOICE); continue; }
-        if (greedy) { if (t == at) taken = c; continue; }
-        bool gone = false;
-        for (int k = 0; k < nref; ++k) gone |= refused[k] == (int)t;
-        const double w = gone ? 0.0 : row.w((int)t);
-        if ((double)v.u_accept[lo + c] * (row.q ? (double)row.q[t] : 1.0) * D < w) { taken = c; continue; }
-        if (row.q) {
-          const double a0 = row.a;
-          row.a += D;
-          double s = 0.0;
-          for (int i = tid; i < V; i += VT) s += row.w(i);
-          s = block_sum_d(s, red);
-          if (s > 0.0) D = s; else row.a = a0;
-        } else if (!gone && D - w > 0.0) {
+        for (int i = 0; i < Pieces<T>::E; ++i) x += w[i];
+      }
+      return exchange(x, &which);
+    };
+    auto make_sure = [&]() {
+      const float* q = left.q;
+      left.q = nullptr; left.nref = 0;
+      S = sum_left();
+      left.q = q;
+      sure = true;
+    };
+    if (!GREEDY && choice) {
+      for (int k = 0; k < nkid && taken < 0; ++k) {
+        const double u = sh.u[sh.kid[k]], qt = sh.kq[k], e = sh.kz[k] > -INFINITY ? exp(((double)sh.kz[k] - left.zmax) * left.invT) : 0.0;
+        bool again = false;                                     // an earlier sibling with this token was refused: nothing is left of it
+        if (!qrow) for (int i = lane; i < k + lane; i += 32) again |= __any_sync(0xffffffffu, i < k && sh.gone[i < k ? i : 0] && sh.token[sh.kid[i < k ? i : 0]] == sh.token[sh.kid[k]]);
+        auto weight = [&]() { const double w = e / S - a * qt; return qrow ? (w > 0.0 ? w : 0.0) : again ? 0.0 : e / S; };
+        double w = weight();
+        if (!sure && (fabs(u * qt * D - w) <= slack * (u * qt + e / S) || (!qrow && D - w < 1e-4))) {
+          const double S0 = S;
+          make_sure();
+          w = weight();
+          if (!qrow) D = 1.0 - (1.0 - D) * (S0 / S);
+        }
+        if (u * qt * D < w) { taken = sh.kid[k]; break; }
+        if (qrow) {
+          a0 = a;
+          a += D;
+          if (k + 1 < nkid) {                                   // (after the last child the sum below does this)
+            if (!sure) { make_sure(); }
+            const double d = sum_left() / S;
+            if (d > 0.0) D = d; else a = a0;
+          }
+        } else if (!again && D - w > 0.0) {
           D -= w;
-          __syncthreads();
-          if (tid == 0) refused[nref] = (int)t;
-          ++nref;
-          __syncthreads();
+          __syncwarp();
+          sh.gone[k] = 1;                                       // every thread of the cluster writes the same into its block's copy
+          __syncwarp();
         }
       }
-    if (choice && taken < 0 && !greedy) {                       // the last token
-      const int per = (V + VT - 1) / VT, i0 = min(V, tid * per), i1 = min(V, i0 + per);
-      auto weight = [&](int i) { for (int k = 0; k < nref; ++k) if (refused[k] == i) return 0.0; return row.w(i); };
-      double s = 0.0;
-      int lastpos = -1;
-      for (int i = i0; i < i1; ++i) { const double w = weight(i); s += w; if (w > 0.0) lastpos = i; }
-      double inc = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(0xffffffffu, inc, o); if ((tid & 31) >= o) inc += y; }
-      __syncthreads();
-      if ((tid & 31) == 31) red[tid >> 5] = inc;
-      if (tid == 0) pick = -1;
-      __syncthreads();
-      double before = 0.0, total = 0.0;
-      for (int k = 0; k < VT / 32; ++k) { if (k < (tid >> 5)) before += red[k]; total += red[k]; }
-      const double goal = (double)v.u_sample[b] * total, excl = before + inc - s;
-      if (lastpos >= 0 && excl <= goal) {                       // the last such chunk holds the index (or rounding put it just before)
-        double run = excl;
-        int hit = lastpos;
-        for (int i = i0; i < i1; ++i) { run += weight(i); if (run > goal) { hit = i; break; } }
-        atomicMax(&pick, hit);
-      }
-      __syncthreads();
-      last = pick;
     }
-    if (tid == 0) {
+    if (taken < 0 && !GREEDY && choice) {                       // the last token
+      if (qrow && !sure && a > 0.0) make_sure();
+      __syncthreads();
+      left.nref = qrow ? 0 : nkid;
+      double total = sum_left();
+      if (!(total > 0.0) && (a > 0.0 || left.nref)) { a = a0; left.nref = 0; total = sum_left(); }
+      // the last segment that begins at or before the goal and is not empty
+      const double goal = (double)v.u_sample[b] * total;
+      constexpr int PER = MAX_CL * VW / 32;
+      double part[PER], inc = 0.0, before = 0.0;
+      int seg = -1;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) { part[i] = lane * PER + i < CL * VW ? sh.sum[which][lane * PER + i] : 0.0; inc += part[i]; }
+      double run = inc;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += y; }
+      run -= inc;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (part[i] > 0.0 && run <= goal) { seg = lane * PER + i; before = run; }
+        run += part[i];
+      }
+      seg = __reduce_max_sync(0xffffffffu, seg);
+      before = __shfl_sync(0xffffffffu, before, max(seg, 0) / PER);
+      if (seg == rank * VW + warp) {                            // that warp looks for the index
+        int hit = -1, lastpos = -1;
+        double at = before;
+        for (int base = j0; base < j1 && hit < 0; base += 32) {
+          double w[Pieces<T>::E], x = 0.0;
+          const int j = base + lane;
+#pragma unroll
+          for (int i = 0; i < Pieces<T>::E; ++i) w[i] = 0.0;
+          if (j < j1) left.weights(j, sh, w);
+#pragma unroll
+          for (int i = 0; i < Pieces<T>::E; ++i) x += w[i];
+          double inc = x;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) { const double y = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += y; }
+          double r = at + inc - x;
+          int mine = -1, pos = -1;
+#pragma unroll
+          for (int i = 0; i < Pieces<T>::E; ++i) {
+            r += w[i];
+            if (w[i] > 0.0) { pos = P.first(j) + i; if (mine < 0 && r > goal) mine = pos; }
+          }
+          const uint32_t any = __ballot_sync(0xffffffffu, mine >= 0), some = __ballot_sync(0xffffffffu, pos >= 0);
+          if (some) lastpos = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
+          if (any) hit = __shfl_sync(0xffffffffu, mine, __ffs(any) - 1);
+          at += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) v.tokens_out[(size_t)b * v.max_out + level] = hit >= 0 ? hit : lastpos;
+      }
+      if (seg < 0 && writer) v.tokens_out[(size_t)b * v.max_out + level] = -1;
+    }
+    if (writer) {
       v.path_out[(size_t)b * v.max_out + level] = lo + node;
-      v.tokens_out[(size_t)b * v.max_out + level] = taken >= 0 ? v.token[lo + taken] : last;
+      if (taken >= 0) v.tokens_out[(size_t)b * v.max_out + level] = sh.token[taken];
+      else if (GREEDY || !choice) v.tokens_out[(size_t)b * v.max_out + level] = choice ? st.at : -1;
     }
     ++level;
     if (taken < 0) break;
     node = taken;
-    __syncthreads();
+    __syncthreads();                                            // the children's arrays are used again
   }
-  if (tid == 0) v.n_out[b] = level;
+  if (writer) v.n_out[b] = level;
+  cl.sync();                                                    // no block leaves while another may still write into its shared memory
+}
+
+template <typename T, bool GREEDY> cudaError_t launch(cudaStream_t st, const VerifyArgs& A) {
+  // blocks of a cluster: 512 pieces of 16 bytes a block (two rounds of its 256 threads) and not more than 16
+  const long long pieces = ((long long)A.v.vocab * (long long)sizeof(T) + 15) / 16;
+  int cl = 1;
+  while (cl < MAX_CL && pieces > cl * 512ll) cl *= 2;
+  if (cl > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)A.v.batch * cl); cfg.blockDim = dim3(VT); cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cl; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_verify<T, GREEDY>, A);
 }
 
 }  // namespace
@@ -185,7 +445,8 @@ extern "C" int pcpb_op_verify_drafts(void* stream, const pcpb_verify* args, int3
   d.on(v.u_accept, "u_accept"); d.on(v.u_sample, "u_sample"); d.on(v.tokens_out, "tokens_out"); d.on(v.path_out, "path_out"); d.on(v.n_out, "n_out");
   d.on(status, "status");
   if (d.enter()) return d.rc;
-  if (v.dtype == PCPB_BF16) k_verify<bf16><<<v.batch, VT, 0, (cudaStream_t)stream>>>(A);
-  else k_verify<float><<<v.batch, VT, 0, (cudaStream_t)stream>>>(A);
-  return d.done(cudaGetLastError());
+  const bool greedy = v.temperature < 1e-6, half = v.dtype == PCPB_BF16;
+  A.ahead = (double)v.n_rows * v.vocab * (half ? 2 : 4) <= AHEAD_BYTES;
+  cudaStream_t st = (cudaStream_t)stream;
+  return d.done(half ? (greedy ? launch<bf16, true>(st, A) : launch<bf16, false>(st, A)) : (greedy ? launch<float, true>(st, A) : launch<float, false>(st, A)));
 }

@@ -402,6 +402,7 @@ long long pcpb_rollout_launch_count(const pcpb_rollout* r);
 #define PCPB_OPS_BAD_LENGTH 2    /* a negative or too large length, start or row number: clipped to what there is */
 #define PCPB_OPS_BAD_TREE 4      /* a parent that does not come before its child: the node counts as a root */
 #define PCPB_OPS_NO_CHOICE 8     /* logits without a finite largest value, or a token outside the vocabulary */
+#define PCPB_OPS_STUCK 16        /* a wait inside a kernel ran out (it never should): the call's results are not valid */
 
 /* One layer's paged cache: page p holds rows [n_kv_head][page_tokens][head_dim] at k + p * page_stride.  Position t of
  * sequence b is row t % page_tokens of page block_table[b * max_pages + t / page_tokens].  dtype PCPB_BF16 holds the rows

@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "decode_ops.h"
+#include "tc_common.cuh"
 
 namespace pcpb {
 namespace {
@@ -468,18 +469,19 @@ template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_t
   }
 }
 
-// Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles), one thread per four columns of a row.
+// Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles, ROWS / 16): a block joins 16 rows.
 template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ AttnArgs A, int blocks) {
   const int b = blockIdx.x;
   const Seq s = seq_of(A, b);
   const int rows = s.n * A.G, RT = (rows + ROWS - 1) / ROWS, T = tiles_of(s.ctx) + tiles_of(s.n);
   const int item = blockIdx.y;
   if (item >= RT * A.c.n_kv_head) return;
+  const int kvh = item / RT, row0 = item % RT * ROWS, r0 = blockIdx.z * 16;
+  if (row0 + r0 >= rows) return;
   const Parts P = parts_of(A.plan[b] + (long long)item * T, T, tile_share(A.plan[A.c.batch], blocks));
   if (P.c0 == P.c1) return;
-  const int kvh = item / RT, row0 = item % RT * ROWS;
-  for (int i = threadIdx.x; i < ROWS * (HD / 4); i += blockDim.x) {
-    const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+  for (int i = threadIdx.x; i < 16 * (HD / 4); i += blockDim.x) {
+    const int r = r0 + i / (HD / 4), c = i % (HD / 4) * 4;
     if (row0 + r >= rows) continue;
     float m = -INFINITY;
     for (int k = P.c0; k <= P.c1; ++k) m = fmaxf(m, A.part_ml[((size_t)part_slot(P, k) * ROWS + r) * 2]);
@@ -498,6 +500,564 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
     if (A.a.lse && c == 0) A.a.lse[(size_t)(s.n0 + node) * A.a.n_head + h] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
   }
+}
+
+// ---- the kernel for many rows: tcgen05.mma ---------------------------------------------------------------------------
+// An item is up to 256 rows (two tiles of 128) of one kv head.  Two streams of score and output tiles are in flight in tensor memory, so that
+// the products of one run while the other's softmax does: with more than 128 rows the streams are the two row tiles, which share
+// every tile of keys; with fewer both streams have the same rows and take the tiles of keys in turn, and are joined at the end.
+//   loaders (4 warps)   find the rows of a tile's 128 positions in the block table, bring keys and values into 128-byte-swizzled shared
+//                       memory as bf16 (8-bit codes are widened on the way, the next half-tile's codes in registers meanwhile), scales
+//                       and the valid positions into a ring of tile descriptions
+//   one warp            issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as the MN-major operand)
+//   softmax (2 x 4)     a thread owns a row: scores from tensor memory, running maximum and sum, weights as bf16 over the scores
+// The reference maximum of a row moves only when a score passes it by 2^8 (weights up to 256 cost nothing: bf16 keeps its relative
+// precision), so the output is rescaled in few tiles.
+// Every wait is bounded.  A wait that runs out marks the block as failed and sets PCPB_OPS_STUCK; from there on waits return at once and all
+// warps run their loops to the end (the same barriers, valid addresses, wrong numbers), so that nothing hangs.
+constexpr int TR = 256;              // rows of an item
+constexpr int TC_THREADS = 13 * 32;
+constexpr int INFO = 4;              // tile descriptions in flight
+
+template <int HD> struct TcCfg {
+  static constexpr int TILE_BYTES = 128 * HD * 2;
+  static constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + 2 * TILE_BYTES, OFF_INFO = OFF_V + 2 * TILE_BYTES;
+  static constexpr int INFO_BYTES = 2 * 128 * 4 + 16;                     // key scales, value scales, valid positions
+  static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2][128] byte offsets of rows
+  static constexpr int OFF_ML = OFF_ROW + 2 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
+  static constexpr int OFF_PAR = OFF_ML + 2 * 128 * 2 * 4;                // parents
+  static constexpr int OFF_BAR = OFF_PAR + MAX_NODES * 2;
+  static constexpr int OFF_PLAN = OFF_BAR + 256;
+  static constexpr int BYTES = OFF_PLAN + (MAX_BATCH + 1) * 8 + 1024;
+  static_assert(BYTES <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, int* fail) {
+  if (!mbar_try(bar, parity) && !*(volatile int*)fail) mbar_wait(bar, parity, fail, 1);
+  __syncwarp();                                                 // what follows is for whole warps
+}
+__device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+// Byte offset of 16-byte piece c of row r in a 128-row tile of 64-column halves, 128-byte swizzle
+__device__ __forceinline__ uint32_t sw_off(int r, int c) { return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+__device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// The blocks' segments: a run of tiles [t0, t1) of one item
+struct Seg { int b, kvh, row0, rows, t0, t1, ct, T; Seq s; };
+__device__ __forceinline__ Seg seg_at(const AttnArgs& A, const long long* plan, long long w, long long w1) {
+  Seg g;
+  g.b = seq_at(plan, A.c.batch, w);
+  g.s = seq_of(A, g.b);
+  g.ct = tiles_of(g.s.ctx); g.T = g.ct + tiles_of(g.s.n);
+  const int all = g.s.n * A.G, RT = (all + TR - 1) / TR;
+  const long long at = w - plan[g.b], item = at / g.T;
+  g.t0 = (int)(at % g.T);
+  g.t1 = (int)min((long long)g.T, g.t0 + (w1 - w));
+  g.kvh = (int)(item / RT); g.row0 = (int)(item % RT) * TR;
+  g.rows = min(TR, all - g.row0);
+  return g;
+}
+
+template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_tree_tc(const __grid_constant__ AttnArgs A) {
+  using Cfg = TcCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sQ = base, sK = base + Cfg::OFF_K, sV = base + Cfg::OFF_V, sBar = base + Cfg::OFF_BAR;
+  long long* plan = reinterpret_cast<long long*>(gen + Cfg::OFF_PLAN);
+  __shared__ int fail;
+  __shared__ uint32_t tmem_slot, odd[4][MAX_NODES / 32];        // odd: nodes of a segment whose values hold an infinity or a NaN (the loaders are at most two segments ahead)
+  auto kfull = [&](int i) { return sBar + 8u * i; };
+  auto kempty = [&](int i) { return sBar + 16u + 8u * i; };
+  auto vfull = [&](int i) { return sBar + 32u + 8u * i; };
+  auto vempty = [&](int i) { return sBar + 48u + 8u * i; };
+  auto sfull = [&](int x) { return sBar + 64u + 8u * x; };
+  auto pfull = [&](int x) { return sBar + 80u + 8u * x; };
+  auto pvdone = [&](int x) { return sBar + 96u + 8u * x; };
+  auto oempty = [&](int x) { return sBar + 112u + 8u * x; };
+  auto ifull = [&](int i) { return sBar + 128u + 8u * i; };
+  auto iempty = [&](int i) { return sBar + 160u + 8u * i; };
+  const uint32_t qfull = sBar + 192u, odone = sBar + 200u;
+
+  const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    fail = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kfull(i), 128); mbar_init(kempty(i), 1); mbar_init(vfull(i), 128); mbar_init(vempty(i), 1);
+      mbar_init(sfull(i), 1); mbar_init(pfull(i), 4); mbar_init(pvdone(i), 1); mbar_init(oempty(i), 8);
+    }
+    for (int i = 0; i < INFO; ++i) { mbar_init(ifull(i), 128); mbar_init(iempty(i), 8); }
+    mbar_init(qfull, 256); mbar_init(odone, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  make_plan<TR>(A, plan);                                       // (its barriers also publish the setup above)
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
+  const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
+  if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
+  const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
+  auto s_col = [&](int x) { return tmem + 128u * x; };
+  auto o_col = [&](int x) { return tmem + 256u + 128u * x; };
+
+  if (warp >= 8 && warp < 12) {
+    // =========================== loaders ===========================
+    const int t = threadIdx.x - 256;
+    constexpr int ES = CODE == PCPB_BF16 ? 2 : 1, PIECES = HD * ES / 16, NP = PIECES;          // 16-byte pieces of a row = pieces of a thread per half-tile
+    long long* rowoff = reinterpret_cast<long long*>(gen + Cfg::OFF_ROW);
+    int gi = 0, seg = 0;                                        // tiles so far (ring positions), segments
+    uint32_t pending = 0;                                       // cp.async path: barrier of the half-tile that is in flight
+    auto flush = [&]() {
+      if (pending) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(pending);
+        pending = 0;
+      }
+    };
+    auto wait_empty = [&](uint32_t bar, uint32_t parity) {
+      if (!mbar_try(bar, parity)) {
+        flush();                                                // what the consumers may need to free the place
+        if (!*(volatile int*)&fail) mbar_wait(bar, parity, &fail, 1);
+      }
+      __syncwarp();
+    };
+    for (long long w = w0; w < w1; ++seg) {
+      const Seg g = seg_at(A, plan, w, w1);
+      const int nt = g.t1 - g.t0;
+      // page and scales of position `t` of a cached tile
+      long long off = -1;
+      float ks = 1.f, vs = 1.f;
+      auto find = [&](int tile) {
+        off = -1; ks = vs = 1.f;
+        const int pos = tile * TILE + t;
+        if (tile >= g.ct || pos >= g.s.ctx) return;
+        const int page = page_of(A.c, g.b, pos / A.c.page_tokens);
+        if (page < 0) { op_note(A.status, PCPB_OPS_BAD_PAGE); return; }
+        off = page_row(page, A.c.page_stride, g.kvh, A.c.page_tokens, pos % A.c.page_tokens, HD) * ES;
+        if (CODE != PCPB_BF16) {
+          const long long so = page_row(page, A.c.scale_stride, g.kvh, A.c.page_tokens, pos % A.c.page_tokens, 1);
+          ks = __ldg(A.c.k_scale + so); vs = __ldg(A.c.v_scale + so);
+        }
+      };
+      uint4 cur[CODE == PCPB_BF16 ? 1 : NP], nxt[CODE == PCPB_BF16 ? 1 : NP];
+      auto fetch = [&](uint4* r, const void* basep, int slot) {  // codes of a half-tile into registers
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+          const long long o = rowoff[slot * 128 + row];
+          r[k] = o < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>((const uint8_t*)basep + o + c * 16));
+        }
+      };
+      auto widen_store = [&](const uint4* r, uint32_t dst) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+          uint32_t p[8];
+          constexpr int CC = CODE == PCPB_BF16 ? PCPB_I8 : CODE;
+          widen4<CC>(r[k].x, p[0], p[1]); widen4<CC>(r[k].y, p[2], p[3]); widen4<CC>(r[k].z, p[4], p[5]); widen4<CC>(r[k].w, p[6], p[7]);
+          const int flip = (c >> 2) & 1;                        // pieces of the second half go the other way round: other banks than the first half's
+          st_shared16(dst + sw_off(row, 2 * c + flip), p[flip ? 4 : 0], p[flip ? 5 : 1], p[flip ? 6 : 2], p[flip ? 7 : 3]);
+          st_shared16(dst + sw_off(row, 2 * c + 1 - flip), p[flip ? 0 : 4], p[flip ? 1 : 5], p[flip ? 2 : 6], p[flip ? 3 : 7]);
+        }
+      };
+      // rows of the nodes (bf16); values that are not numbers are left out and their nodes marked
+      auto node_rows = [&](const bf16* basep, long long row_stride, long long head_stride, int tile, uint32_t dst, bool values) {
+        constexpr int PB = HD / 8;
+        const int n0 = (tile - g.ct) * TILE;
+        for (int idx = t; idx < 128 * PB; idx += 128) {
+          const int row = idx / PB, c = idx % PB, node = n0 + row;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (node < g.s.n) v = *reinterpret_cast<const uint4*>(basep + (long long)(g.s.n0 + node) * row_stride + (long long)g.kvh * head_stride + c * 8);
+          if (values) {
+            uint32_t q[4] = {v.x, v.y, v.z, v.w};
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((q[i] & 0x7F80u) == 0x7F80u) { q[i] &= 0xFFFF0000u; bad = true; }
+              if ((q[i] & 0x7F800000u) == 0x7F800000u) { q[i] &= 0x0000FFFFu; bad = true; }
+            }
+            if (bad) atomicOr(&odd[seg & 3][(node >> 5) & 7], 1u << (node & 31));
+            v = make_uint4(q[0], q[1], q[2], q[3]);
+          }
+          st_shared16(dst + sw_off(row, c), v.x, v.y, v.z, v.w);
+        }
+      };
+      find(g.t0);
+      for (int i = 0; i < nt; ++i, ++gi) {
+        const int tile = g.t0 + i, st = gi & 1, in = gi % INFO, slot = gi & 1;
+        const bool cached = tile < g.ct;
+        // description of the tile
+        wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
+        float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
+        info[t] = ks; info[128 + t] = vs;
+        const uint32_t valid = __ballot_sync(0xffffffffu, off >= 0);
+        if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
+        mbar_arrive(ifull(in));
+        if (i == 0 || CODE == PCPB_BF16) {                      // (8-bit: later tiles' rows were published with the tile before)
+          rowoff[slot * 128 + t] = off;
+          bar_sync(2, 128);
+        }
+        const uint32_t kdst = sK + st * Cfg::TILE_BYTES, vdst = sV + st * Cfg::TILE_BYTES;
+        const uint32_t ephase = ((gi >> 1) & 1) ^ 1;
+        if (CODE == PCPB_BF16 && cached) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t dst = h ? vdst : kdst;
+            const uint8_t* src = (const uint8_t*)(h ? A.c.v : A.c.k);
+            wait_empty(h ? vempty(st) : kempty(st), ephase);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+              const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+              const long long o = rowoff[slot * 128 + row];
+              cp_async16z(dst + sw_off(row, c), src + (o < 0 ? 0 : o + c * 16), o >= 0);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (pending) {
+              asm volatile("cp.async.wait_group 1;" ::: "memory");
+              fence_proxy_async_smem();
+              mbar_arrive(pending);
+            }
+            pending = h ? vfull(st) : kfull(st);
+            if (h == 0) find(tile + 1);                         // the next tile's pages, while this one's rows are on their way
+          }
+        } else if (CODE != PCPB_BF16 && cached) {
+          if (i == 0) fetch(cur, A.c.k, slot);
+          fetch(nxt, A.c.v, slot);
+          find(tile + 1);
+          wait_empty(kempty(st), ephase);
+          widen_store(cur, kdst);
+          fence_proxy_async_smem();
+          mbar_arrive(kfull(st));
+          if (i + 1 < nt) {
+            rowoff[(slot ^ 1) * 128 + t] = off;
+            bar_sync(2, 128);
+            if (tile + 1 < g.ct) fetch(cur, A.c.k, slot ^ 1);
+          }
+          wait_empty(vempty(st), ephase);
+          widen_store(nxt, vdst);
+          fence_proxy_async_smem();
+          mbar_arrive(vfull(st));
+        } else {
+          wait_empty(kempty(st), ephase);
+          node_rows((const bf16*)A.a.k, A.a.k_row, A.a.k_head, tile, kdst, false);
+          fence_proxy_async_smem();
+          mbar_arrive(kfull(st));
+          wait_empty(vempty(st), ephase);
+          if (t < MAX_NODES / 32 && tile == max(g.ct, g.t0)) odd[seg & 3][t] = 0u;
+          bar_sync(2, 128);
+          node_rows((const bf16*)A.a.v, A.a.v_row, A.a.v_head, tile, vdst, true);
+          fence_proxy_async_smem();
+          mbar_arrive(vfull(st));
+          off = -1; ks = vs = 1.f;
+          if (CODE != PCPB_BF16 && i + 1 < nt) { rowoff[(slot ^ 1) * 128 + t] = off; bar_sync(2, 128); }
+        }
+      }
+      w += nt;
+    }
+    flush();
+  } else if (warp == 12) {
+    // =========================== MMA issuer ===========================
+    constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    int gi = 0, seg = 0;
+    int pv[2] = {0, 0};                                         // output products of a stream so far
+    for (long long w = w0; w < w1; ++seg) {
+      const Seg g = seg_at(A, plan, w, w1);
+      const int nt = g.t1 - g.t0;
+      const bool pair = g.rows > 128;
+      const int cnt[2] = {pair ? nt : (nt + 1) / 2, pair ? nt : nt / 2};
+      wait(qfull, seg & 1, &fail);
+      tc_fence_after();
+      auto qk = [&](int x, int j) {
+        const int i = gi + (pair ? j : 2 * j + x), st = i & 1;
+        wait(kfull(st), (i >> 1) & 1, &fail);
+        tc_fence_after();
+        const uint32_t a = sQ + (pair ? x * Cfg::TILE_BYTES : 0), b = sK + st * Cfg::TILE_BYTES;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t o = (uint32_t)(k >> 2) * 16384u + (uint32_t)(k & 3) * 32u;
+          mma_bf16_elect(s_col(x), make_desc(a + o, 16, 1024), make_desc(b + o, 16, 1024), ID_S, k > 0);
+        }
+        mma_commit_elect(sfull(x));
+        if (!pair || x == 1) mma_commit_elect(kempty(st));
+      };
+      if (cnt[0] > 0) qk(0, 0);
+      if (cnt[1] > 0) qk(1, 0);
+      for (int j = 0; j < cnt[0]; ++j) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (j >= cnt[x]) continue;
+          const int i = gi + (pair ? j : 2 * j + x), st = i & 1;
+          wait(pfull(x), pv[x] & 1, &fail);
+          wait(vfull(st), (i >> 1) & 1, &fail);
+          if (j == 0) wait(oempty(x), (seg & 1) ^ 1, &fail);    // the last segment's output has been read
+          tc_fence_after();
+          const uint32_t b = sV + st * Cfg::TILE_BYTES;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_bf16_ts_elect(o_col(x), s_col(x) + 8u * k, make_desc(b + k * 2048u, 16384, 1024), ID_O, j > 0 || k > 0);
+          mma_commit_elect(pvdone(x));
+          if (!pair || x == 1) mma_commit_elect(vempty(st));
+          ++pv[x];
+          if (j + 1 < cnt[x]) qk(x, j + 1);
+        }
+      }
+      mma_commit_elect(odone);
+      gi += nt;
+      w += nt;
+    }
+  } else {
+    // =========================== softmax ===========================
+    const int x = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    const float zscale = A.a.scale * LOG2E;
+    int gi = 0, seg = 0, sn = 0;                                // tiles, segments; score tiles of this stream so far
+    int16_t* par = reinterpret_cast<int16_t*>(gen + Cfg::OFF_PAR);
+    float* ml = reinterpret_cast<float*>(gen + Cfg::OFF_ML);
+    for (long long w = w0; w < w1; ++seg) {
+      const Seg g = seg_at(A, plan, w, w1);
+      const int nt = g.t1 - g.t0;
+      const bool pair = g.rows > 128;
+      const int tr = pair ? x * 128 + r : r;                    // row of the item
+      const bool live = tr < g.rows, warp_live = (pair ? x * 128 : 0) + q4 * 32 < g.rows;
+      const int node = (g.row0 + tr) / A.G, head = g.kvh * A.G + (g.row0 + tr) % A.G;
+      {
+        const bf16* src = (const bf16*)A.a.q + (long long)(g.s.n0 + node) * A.a.q_row + (long long)head * A.a.q_head;
+        const uint32_t dst = sQ + (pair ? x * Cfg::TILE_BYTES : 0);
+        const int c0 = pair ? 0 : x * (HD / 16), c1 = pair ? HD / 8 : c0 + HD / 16;
+        for (int c = c0; c < c1; ++c) {
+          const uint4 v = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          st_shared16(dst + sw_off(r, c), v.x, v.y, v.z, v.w);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(qfull);
+      }
+      const bool has_tree = g.t1 > g.ct;
+      uint32_t anc[MAX_NODES / 32] = {};
+      if (has_tree) {
+        for (int i = threadIdx.x; i < g.s.n; i += 256) {
+          int bad = 0;
+          par[i] = (int16_t)clip_parent(A.a.parent ? A.a.parent[g.s.n0 + i] : i - 1, i, &bad);
+          if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
+        }
+        bar_sync(1, 256);
+        int i = live ? node : -1;
+        while (i >= 0) {
+#pragma unroll
+          for (int k = 0; k < MAX_NODES / 32; ++k) anc[k] |= (i >> 5) == k ? 1u << (i & 31) : 0u;
+          i = par[i];
+        }
+      }
+      float mref = -INFINITY, l = 0.f;
+      int done = 0;                                             // tiles of this stream in this segment
+      for (int i = pair ? 0 : x; i < nt; i += pair ? 1 : 2, ++done, ++sn) {
+        const int in = (gi + i) % INFO;
+        wait(ifull(in), ((gi + i) / INFO) & 1, &fail);
+        wait(sfull(x), sn & 1, &fail);
+        tc_fence_after();
+        if (warp_live) {
+          const float* info = reinterpret_cast<const float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
+          const int tile = g.t0 + i;
+          const bool tree = tile >= g.ct;
+          uint32_t see[4];
+          if (tree) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) see[k] = tile == g.ct ? anc[k] : anc[4 + k];
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) see[k] = reinterpret_cast<const uint32_t*>(info)[256 + k];
+          }
+          const int own = tree && A.a.null_self ? node - (tile - g.ct) * TILE : -1;
+          const bool all = __all_sync(0xffffffffu, (see[0] & see[1] & see[2] & see[3]) == 0xffffffffu && own < 0);
+          // largest score
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+            if (all) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                float f[4] = {1.f, 1.f, 1.f, 1.f};
+                if (CODE != PCPB_BF16) { const float4 k4 = *reinterpret_cast<const float4*>(info + 32 * c + j); f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w; }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, __uint_as_float(v[j + k]) * (zscale * f[k]));
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float z = __uint_as_float(v[j]) * (zscale * info[32 * c + j]);
+                if (32 * c + j == own) z = 0.f;
+                if ((see[c] >> j) & 1u) mx = fmaxf(mx, z);
+              }
+            }
+          }
+          // move the reference maximum
+          const bool up = mx > mref + 8.f || (mref == -INFINITY && mx > -INFINITY);
+          if (__any_sync(0xffffffffu, up)) {
+            const float ref = up ? mx : mref;
+            const float corr = up && mref > -INFINITY ? ex2(mref - ref) : 1.f;
+            if (done > 0) {
+              wait(pvdone(x), (sn - 1) & 1, &fail);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32(o_col(x) + lane_off + 32u * c, v);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t u[16];
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(v[16 * h + j]) * corr);
+                  tmem_st16(o_col(x) + lane_off + 32u * c + 16u * h, u);
+                }
+              }
+              tmem_st_wait();
+            }
+            l *= corr;
+            mref = ref;
+          }
+          const float ref = mref == -INFINITY ? 0.f : mref;
+          // weights
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], p[16];
+            tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+            if (all) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                float f[4] = {1.f, 1.f, 1.f, 1.f}, h[4] = {1.f, 1.f, 1.f, 1.f}, e[4];
+                if (CODE != PCPB_BF16) {
+                  const float4 k4 = *reinterpret_cast<const float4*>(info + 32 * c + j), v4 = *reinterpret_cast<const float4*>(info + 128 + 32 * c + j);
+                  f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w;
+                  h[0] = v4.x; h[1] = v4.y; h[2] = v4.z; h[3] = v4.w;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  e[k] = ex2(fmaf(__uint_as_float(v[j + k]), zscale * f[k], -ref));
+                  l += e[k];
+                  if (CODE != PCPB_BF16) e[k] *= h[k];
+                }
+                p[j / 2] = pack2(e[0], e[1]); p[j / 2 + 1] = pack2(e[2], e[3]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float z = __uint_as_float(v[j]) * (zscale * info[32 * c + j]);
+                if (32 * c + j == own) z = 0.f;
+                float e = (see[c] >> j) & 1u ? ex2(z - ref) : 0.f;
+                l += e;
+                e = (see[c] >> j) & 1u && 32 * c + j != own ? e * info[128 + 32 * c + j] : 0.f;
+                if (j & 1) p[j / 2] = pack2(__uint_as_float(p[j / 2]), e); else p[j / 2] = __float_as_uint(e);
+              }
+            }
+            tmem_st16(s_col(x) + lane_off + 16u * c, p);
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(pfull(x));
+          mbar_arrive_n(iempty(in), pair ? 1u : 2u);
+        }
+      }
+      // the segment's end: outputs of both streams are complete
+      wait(odone, seg & 1, &fail);
+      tc_fence_after();
+      if (!pair) {
+        ml[(x * 128 + r) * 2] = mref; ml[(x * 128 + r) * 2 + 1] = l;
+        bar_sync(1, 256);
+      }
+      if (warp_live) {
+        float f0 = 1.f, f1 = 0.f;
+        __syncwarp();
+        const bool two = !pair && nt > 1;                       // the second stream had tiles
+        if (!pair) {
+          const float m0 = ml[r * 2], l0 = ml[r * 2 + 1], m1 = two ? ml[(128 + r) * 2] : -INFINITY, l1 = two ? ml[(128 + r) * 2 + 1] : 0.f;
+          mref = fmaxf(m0, m1);
+          const float ref = mref == -INFINITY ? 0.f : mref;
+          f0 = ex2(m0 - ref); f1 = ex2(m1 - ref);
+          l = f0 * l0 + f1 * l1;
+        }
+        const bool whole = g.t0 == 0 && g.t1 == g.T;
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const size_t slot = (size_t)blockIdx.x * 2 + (w == w0 ? 0 : 1);
+        bf16* dst = (bf16*)A.a.out + (long long)(g.s.n0 + node) * A.a.out_row + (long long)head * A.a.out_head;
+        float* part = A.part_o + (slot * TR + tr) * HD;
+        bool strange = false;
+        if (has_tree) {
+#pragma unroll
+          for (int k = 0; k < MAX_NODES / 32; ++k) strange |= (anc[k] & odd[seg & 3][k]) != 0u;
+        }
+        // columns: with two row tiles all of the row's; else the warps of the two groups take half of them each
+        const int c0 = pair ? 0 : x * (HD / 32), c1 = pair ? HD / 16 : c0 + HD / 32;
+#pragma unroll 1
+        for (int c = c0; c < c1; ++c) {
+          uint32_t v[16], u[16];
+          __syncwarp();
+          tmem_ld16_issue(o_col(pair ? x : 0) + lane_off + 16u * c, v);
+          if (two) tmem_ld16_issue(o_col(1) + lane_off + 16u * c, u);
+          tmem_ld_wait16(v);
+          if (two) tmem_ld_wait16(u);
+          float o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            o[j] = __uint_as_float(v[j]) * f0;
+            if (two) o[j] = fmaf(__uint_as_float(u[j]), f1, o[j]);
+          }
+          if (strange)                                          // infinities and NaN of the values this row does attend
+            for (int i = max(0, g.t0 - g.ct) * TILE; i < min(g.s.n, (g.t1 - g.ct) * TILE); ++i) {
+              uint32_t word = 0;
+#pragma unroll
+              for (int k = 0; k < MAX_NODES / 32; ++k) word = (i >> 5) == k ? anc[k] & odd[seg & 3][k] : word;
+              if (!((word >> (i & 31)) & 1u) || (A.a.null_self && i == node)) continue;
+              const bf16* vr = (const bf16*)A.a.v + (long long)(g.s.n0 + i) * A.a.v_row + (long long)g.kvh * A.a.v_head + 16 * c;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) { const float y = to_f(vr[j]); if (!isfinite(y)) o[j] += y; }
+            }
+          if (live && whole) {
+            uint32_t p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = pack2(o[2 * j] * inv, o[2 * j + 1] * inv);
+            *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(p[0], p[1], p[2], p[3]);
+            *reinterpret_cast<uint4*>(dst + 16 * c + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+          } else if (live) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(part + 16 * c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        if (live && (pair || x == 0)) {
+          if (whole) { if (A.a.lse) A.a.lse[(size_t)(g.s.n0 + node) * A.a.n_head + head] = l == 0.f ? -INFINITY : mref * LN2 + logf(l); }
+          else { A.part_ml[(slot * TR + tr) * 2] = mref; A.part_ml[(slot * TR + tr) * 2 + 1] = l; }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(oempty(0)); mbar_arrive(oempty(1)); }
+      bar_sync(1, 256);                                         // ml, par and q are used again
+      gi += nt;
+      w += nt;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && fail) op_note(A.status, PCPB_OPS_STUCK);
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -534,10 +1094,26 @@ template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnA
   k_tree_join<HD, RW><<<dim3(A.c.batch, items), 256, 0, st>>>(A, blocks);
   return cudaGetLastError();
 }
+template <int HD, int CODE> cudaError_t launch_tc(cudaStream_t st, const AttnArgs& A, int blocks) {
+  cudaError_t e = cudaFuncSetAttribute(k_tree_tc<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HD>::BYTES);
+  if (e != cudaSuccess) return e;
+  k_tree_tc<HD, CODE><<<blocks, TC_THREADS, TcCfg<HD>::BYTES, st>>>(A);
+  const int rows = A.a.max_nodes * A.G, items = A.c.n_kv_head * ((rows + TR - 1) / TR);
+  k_tree_join<HD, TR><<<dim3(A.c.batch, items, (min(rows, TR) + 15) / 16), 256, 0, st>>>(A, blocks);
+  return cudaGetLastError();
+}
+// Rows of a kv head from which on the tensor-core kernel takes over
+constexpr int TC_FROM = 17;
+bool use_tc(const pcpb_kv_cache& c, int G, int max_nodes) { return c.head_dim != 32 && max_nodes * G >= TC_FROM; }
+template <int HD, int CODE> cudaError_t launch_any(cudaStream_t st, const AttnArgs& A, int blocks) {
+  if constexpr (HD != 32)
+    if (use_tc(A.c, A.G, A.a.max_nodes)) return launch_tc<HD, CODE>(st, A, blocks);
+  return launch_rows<HD, CODE>(st, A, blocks);
+}
 template <int HD> cudaError_t launch_code(cudaStream_t st, const AttnArgs& A, int blocks) {
-  if (A.c.dtype == PCPB_BF16) return launch_rows<HD, PCPB_BF16>(st, A, blocks);
-  if (A.c.dtype == PCPB_I8) return launch_rows<HD, PCPB_I8>(st, A, blocks);
-  return launch_rows<HD, PCPB_E4M3>(st, A, blocks);
+  if (A.c.dtype == PCPB_BF16) return launch_any<HD, PCPB_BF16>(st, A, blocks);
+  if (A.c.dtype == PCPB_I8) return launch_any<HD, PCPB_I8>(st, A, blocks);
+  return launch_any<HD, PCPB_E4M3>(st, A, blocks);
 }
 
 }  // namespace
@@ -549,7 +1125,7 @@ extern "C" size_t pcpb_op_tree_attention_workspace(int device, const pcpb_kv_cac
   if (err && cap) err[0] = 0;
   pcpb_kv_cache c;
   if (check_cache(cache, &c, err, cap) || check_heads(c, n_head, max_nodes, err, cap)) return 0;
-  return layout(c, sm_count(device), RW).bytes;
+  return layout(c, sm_count(device), use_tc(c, n_head / c.n_kv_head, max_nodes) ? TR : RW).bytes;
 }
 
 extern "C" int pcpb_op_tree_attention(void* stream, const pcpb_kv_cache* cache, const pcpb_tree_attn* args, int32_t* status, char* err, size_t cap) {
@@ -575,7 +1151,7 @@ extern "C" int pcpb_op_tree_attention(void* stream, const pcpb_kv_cache* cache, 
   d.on(a.ctx_len, "ctx_len"); d.on(a.workspace, "workspace"); d.on(status, "status");
   if (d.enter()) return d.rc;
   const int blocks = sm_count(d.dev);
-  const Layout L = layout(A.c, blocks, RW);
+  const Layout L = layout(A.c, blocks, use_tc(A.c, A.G, a.max_nodes) ? TR : RW);
   if (a.workspace_bytes < L.bytes)
     return op_fail(err, cap, PCPB_E_INVALID, "workspace of %zu bytes, %zu are needed (pcpb_op_tree_attention_workspace)", a.workspace_bytes, L.bytes);
   uint8_t* ws = (uint8_t*)a.workspace;

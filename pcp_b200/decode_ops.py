@@ -19,7 +19,7 @@ import ctypes as C
 from .backend import BF16, F32, BackendError, E_INVALID, load_library
 
 I8, E4M3 = 16, 17
-OPS_BAD_PAGE, OPS_BAD_LENGTH, OPS_BAD_TREE, OPS_NO_CHOICE = 1, 2, 4, 8
+OPS_BAD_PAGE, OPS_BAD_LENGTH, OPS_BAD_TREE, OPS_NO_CHOICE, OPS_STUCK = 1, 2, 4, 8, 16
 TREE_MAX_NODES, TREE_MAX_BATCH = 256, 1024
 _ERR_CAP = 256
 

@@ -506,25 +506,30 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
 // An item is up to 256 rows (two tiles of 128) of one kv head.  Two streams of score and output tiles are in flight in tensor memory, so that
 // the products of one run while the other's softmax does: with more than 128 rows the streams are the two row tiles, which share
 // every tile of keys; with fewer both streams have the same rows and take the tiles of keys in turn, and are joined at the end.
-//   loaders (4 warps)   find the rows of a tile's 128 positions in the block table, bring keys and values into 128-byte-swizzled shared
-//                       memory as bf16 (8-bit codes are widened on the way, the next half-tile's codes in registers meanwhile), scales
-//                       and the valid positions into a ring of tile descriptions
-//   one warp            issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as the MN-major operand)
-//   softmax (2 x 4)     a thread owns a row: scores from tensor memory, running maximum and sum, weights as bf16 over the scores
+//   loaders (4 warps for keys, 4 for values)   find the rows of a tile's 128 positions in the block table, two tiles ahead, and bring them into
+//                       128-byte-swizzled shared memory as bf16.  8-bit codes are widened on the way: a thread holds its pieces of
+//                       the next tile in registers and loads a piece of the tile after as soon as it has widened one.  The key
+//                       loaders also describe the tile (scales, valid positions) in a ring.
+//   softmax (2 x 4)     a thread owns a row: scores from tensor memory, running maximum and sum, weights as bf16 over the scores.  The first
+//                       warp of each stream also issues its products when the four warps' weights are there: O += P V (P in tensor
+//                       memory, V as the MN-major operand), then S = Q K^T of the stream's next tile; it would only wait for them
+//                       otherwise, and a warp of its own for it would cost the loaders the registers that hold their codes.
 // The reference maximum of a row moves only when a score passes it by 2^8 (weights up to 256 cost nothing: bf16 keeps its relative
 // precision), so the output is rescaled in few tiles.
+// Loops over a tile's columns are not unrolled further than 64: with everything unrolled the five roles' code did not fit the instruction
+// caches (a third of the stalls were missing instructions).
 // Every wait is bounded.  A wait that runs out marks the block as failed and sets PCPB_OPS_STUCK; from there on waits return at once and all
 // warps run their loops to the end (the same barriers, valid addresses, wrong numbers), so that nothing hangs.
 constexpr int TR = 256;              // rows of an item
-constexpr int TC_THREADS = 13 * 32;
+constexpr int TC_THREADS = 512;      // 128 registers a thread
 constexpr int INFO = 4;              // tile descriptions in flight
 
 template <int HD> struct TcCfg {
   static constexpr int TILE_BYTES = 128 * HD * 2;
   static constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + 2 * TILE_BYTES, OFF_INFO = OFF_V + 2 * TILE_BYTES;
   static constexpr int INFO_BYTES = 2 * 128 * 4 + 16;                     // key scales, value scales, valid positions
-  static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2][128] byte offsets of rows
-  static constexpr int OFF_ML = OFF_ROW + 2 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
+  static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2 loader groups][2][128] byte offsets of rows
+  static constexpr int OFF_ML = OFF_ROW + 4 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
   static constexpr int OFF_PAR = OFF_ML + 2 * 128 * 2 * 4;                // parents
   static constexpr int OFF_BAR = OFF_PAR + MAX_NODES * 2;
   static constexpr int OFF_PLAN = OFF_BAR + 256;
@@ -581,7 +586,6 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
   auto sfull = [&](int x) { return sBar + 64u + 8u * x; };
   auto pfull = [&](int x) { return sBar + 80u + 8u * x; };
   auto pvdone = [&](int x) { return sBar + 96u + 8u * x; };
-  auto oempty = [&](int x) { return sBar + 112u + 8u * x; };
   auto ifull = [&](int i) { return sBar + 128u + 8u * i; };
   auto iempty = [&](int i) { return sBar + 160u + 8u * i; };
   const uint32_t qfull = sBar + 192u, odone = sBar + 200u;
@@ -590,14 +594,14 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
   if (threadIdx.x == 0) {
     fail = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(kfull(i), 128); mbar_init(kempty(i), 1); mbar_init(vfull(i), 128); mbar_init(vempty(i), 1);
-      mbar_init(sfull(i), 1); mbar_init(pfull(i), 4); mbar_init(pvdone(i), 1); mbar_init(oempty(i), 8);
+      mbar_init(kfull(i), 128); mbar_init(kempty(i), 2); mbar_init(vfull(i), 128); mbar_init(vempty(i), 2);
+      mbar_init(sfull(i), 1); mbar_init(pfull(i), 4); mbar_init(pvdone(i), 1);
     }
     for (int i = 0; i < INFO; ++i) { mbar_init(ifull(i), 128); mbar_init(iempty(i), 8); }
-    mbar_init(qfull, 256); mbar_init(odone, 1);
+    mbar_init(qfull, 256); mbar_init(odone, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -612,13 +616,19 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
   auto s_col = [&](int x) { return tmem + 128u * x; };
   auto o_col = [&](int x) { return tmem + 256u + 128u * x; };
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8) {
     // =========================== loaders ===========================
-    const int t = threadIdx.x - 256;
-    constexpr int ES = CODE == PCPB_BF16 ? 2 : 1, PIECES = HD * ES / 16, NP = PIECES;          // 16-byte pieces of a row = pieces of a thread per half-tile
-    long long* rowoff = reinterpret_cast<long long*>(gen + Cfg::OFF_ROW);
+    const bool vals = warp >= 12;                               // this group's operand
+    const int t = threadIdx.x & 127, bar = vals ? 3 : 2;
+    constexpr int ES = CODE == PCPB_BF16 ? 2 : 1, PIECES = HD * ES / 16, NP = PIECES;          // 16-byte pieces of a row = pieces of a thread per tile
+    constexpr int PB = HD / 8;                                  // pieces of a node's row (bf16)
+    long long* rowoff = reinterpret_cast<long long*>(gen + Cfg::OFF_ROW) + (vals ? 256 : 0);
+    const uint8_t* const pages = (const uint8_t*)(vals ? A.c.v : A.c.k);
+    const bf16* const nodes = (const bf16*)(vals ? A.a.v : A.a.k);
+    const long long node_row = vals ? A.a.v_row : A.a.k_row, node_head = vals ? A.a.v_head : A.a.k_head;
+    const uint32_t full0 = vals ? vfull(0) : kfull(0), empty0 = vals ? vempty(0) : kempty(0), dst0 = vals ? sV : sK;
     int gi = 0, seg = 0;                                        // tiles so far (ring positions), segments
-    uint32_t pending = 0;                                       // cp.async path: barrier of the half-tile that is in flight
+    uint32_t pending = 0;                                       // cp.async path: barrier of the tile that is in flight
     auto flush = [&]() {
       if (pending) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -637,193 +647,144 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     for (long long w = w0; w < w1; ++seg) {
       const Seg g = seg_at(A, plan, w, w1);
       const int nt = g.t1 - g.t0;
-      // page and scales of position `t` of a cached tile
-      long long off = -1;
-      float ks = 1.f, vs = 1.f;
-      auto find = [&](int tile) {
-        off = -1; ks = vs = 1.f;
+      // Position t of a cached tile, in three steps a tile apart, so that no load is waited for: the block-table entry, then the row's
+      // place and its scales, then both are used.
+      struct Entry { int raw, in; };
+      struct Found { long long off; float ks, vs; };
+      auto look = [&](int tile) {
         const int pos = tile * TILE + t;
-        if (tile >= g.ct || pos >= g.s.ctx) return;
-        const int page = page_of(A.c, g.b, pos / A.c.page_tokens);
-        if (page < 0) { op_note(A.status, PCPB_OPS_BAD_PAGE); return; }
-        off = page_row(page, A.c.page_stride, g.kvh, A.c.page_tokens, pos % A.c.page_tokens, HD) * ES;
-        if (CODE != PCPB_BF16) {
-          const long long so = page_row(page, A.c.scale_stride, g.kvh, A.c.page_tokens, pos % A.c.page_tokens, 1);
-          ks = __ldg(A.c.k_scale + so); vs = __ldg(A.c.v_scale + so);
+        Entry e{-1, -1};
+        if (tile < min(g.ct, g.t1) && pos < g.s.ctx) {
+          const int lp = pos / A.c.page_tokens;
+          e.in = pos - lp * A.c.page_tokens;
+          e.raw = __ldg(A.c.block_table + (size_t)g.b * A.c.max_pages + lp);       // lp < max_pages: ctx is clipped to the table
         }
+        return e;
       };
-      uint4 cur[CODE == PCPB_BF16 ? 1 : NP], nxt[CODE == PCPB_BF16 ? 1 : NP];
-      auto fetch = [&](uint4* r, const void* basep, int slot) {  // codes of a half-tile into registers
-#pragma unroll
-        for (int k = 0; k < NP; ++k) {
-          const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
-          const long long o = rowoff[slot * 128 + row];
-          r[k] = o < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>((const uint8_t*)basep + o + c * 16));
-        }
-      };
-      auto widen_store = [&](const uint4* r, uint32_t dst) {
-#pragma unroll
-        for (int k = 0; k < NP; ++k) {
-          const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
-          uint32_t p[8];
-          constexpr int CC = CODE == PCPB_BF16 ? PCPB_I8 : CODE;
-          widen4<CC>(r[k].x, p[0], p[1]); widen4<CC>(r[k].y, p[2], p[3]); widen4<CC>(r[k].z, p[4], p[5]); widen4<CC>(r[k].w, p[6], p[7]);
-          const int flip = (c >> 2) & 1;                        // pieces of the second half go the other way round: other banks than the first half's
-          st_shared16(dst + sw_off(row, 2 * c + flip), p[flip ? 4 : 0], p[flip ? 5 : 1], p[flip ? 6 : 2], p[flip ? 7 : 3]);
-          st_shared16(dst + sw_off(row, 2 * c + 1 - flip), p[flip ? 0 : 4], p[flip ? 1 : 5], p[flip ? 2 : 6], p[flip ? 3 : 7]);
-        }
-      };
-      // rows of the nodes (bf16); values that are not numbers are left out and their nodes marked
-      auto node_rows = [&](const bf16* basep, long long row_stride, long long head_stride, int tile, uint32_t dst, bool values) {
-        constexpr int PB = HD / 8;
-        const int n0 = (tile - g.ct) * TILE;
-        for (int idx = t; idx < 128 * PB; idx += 128) {
-          const int row = idx / PB, c = idx % PB, node = n0 + row;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (node < g.s.n) v = *reinterpret_cast<const uint4*>(basep + (long long)(g.s.n0 + node) * row_stride + (long long)g.kvh * head_stride + c * 8);
-          if (values) {
-            uint32_t q[4] = {v.x, v.y, v.z, v.w};
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if ((q[i] & 0x7F80u) == 0x7F80u) { q[i] &= 0xFFFF0000u; bad = true; }
-              if ((q[i] & 0x7F800000u) == 0x7F800000u) { q[i] &= 0x0000FFFFu; bad = true; }
-            }
-            if (bad) atomicOr(&odd[seg & 3][(node >> 5) & 7], 1u << (node & 31));
-            v = make_uint4(q[0], q[1], q[2], q[3]);
+      auto find = [&](const Entry& e) {
+        Found f{-1, 1.f, 1.f};
+        const int page = clip_page(e.raw, A.c.n_pages);
+        if (e.in >= 0 && page < 0) op_note(A.status, PCPB_OPS_BAD_PAGE);
+        if (page >= 0) {
+          f.off = page_row(page, A.c.page_stride, g.kvh, A.c.page_tokens, e.in, HD) * ES;
+          if (CODE != PCPB_BF16 && !vals) {
+            const long long so = page_row(page, A.c.scale_stride, g.kvh, A.c.page_tokens, e.in, 1);
+            f.ks = __ldg(A.c.k_scale + so); f.vs = __ldg(A.c.v_scale + so);
           }
-          st_shared16(dst + sw_off(row, c), v.x, v.y, v.z, v.w);
         }
+        return f;
       };
-      find(g.t0);
-      for (int i = 0; i < nt; ++i, ++gi) {
-        const int tile = g.t0 + i, st = gi & 1, in = gi % INFO, slot = gi & 1;
-        const bool cached = tile < g.ct;
-        // description of the tile
-        wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
-        float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
-        info[t] = ks; info[128 + t] = vs;
-        const uint32_t valid = __ballot_sync(0xffffffffu, off >= 0);
-        if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
-        mbar_arrive(ifull(in));
-        if (i == 0 || CODE == PCPB_BF16) {                      // (8-bit: later tiles' rows were published with the tile before)
-          rowoff[slot * 128 + t] = off;
-          bar_sync(2, 128);
-        }
-        const uint32_t kdst = sK + st * Cfg::TILE_BYTES, vdst = sV + st * Cfg::TILE_BYTES;
-        const uint32_t ephase = ((gi >> 1) & 1) ^ 1;
-        if (CODE == PCPB_BF16 && cached) {
+      auto piece = [&](int k, int slot) {                       // piece k of this thread of a cached tile
+        const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+        const long long o = rowoff[slot * 128 + row];
+        return o < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>(pages + o + c * 16));
+      };
+      uint4 cur[CODE == PCPB_BF16 ? 1 : NP];
+      Entry e1 = look(g.t0), e2 = look(g.t0 + 1);
+      Found f0 = find(e1), f1 = find(e2);                       // of this tile and the next
+      e2 = look(g.t0 + 2);
+      rowoff[(gi & 1) * 128 + t] = f0.off;
+      bar_sync(bar, 128);
+      if (CODE != PCPB_BF16 && g.t0 < g.ct) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) cur[k] = piece(k, gi & 1);
+      }
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t dst = h ? vdst : kdst;
-            const uint8_t* src = (const uint8_t*)(h ? A.c.v : A.c.k);
-            wait_empty(h ? vempty(st) : kempty(st), ephase);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) {
-              const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
-              const long long o = rowoff[slot * 128 + row];
-              cp_async16z(dst + sw_off(row, c), src + (o < 0 ? 0 : o + c * 16), o >= 0);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (pending) {
-              asm volatile("cp.async.wait_group 1;" ::: "memory");
-              fence_proxy_async_smem();
-              mbar_arrive(pending);
-            }
-            pending = h ? vfull(st) : kfull(st);
-            if (h == 0) find(tile + 1);                         // the next tile's pages, while this one's rows are on their way
-          }
-        } else if (CODE != PCPB_BF16 && cached) {
-          if (i == 0) fetch(cur, A.c.k, slot);
-          fetch(nxt, A.c.v, slot);
-          find(tile + 1);
-          wait_empty(kempty(st), ephase);
-          widen_store(cur, kdst);
-          fence_proxy_async_smem();
-          mbar_arrive(kfull(st));
-          if (i + 1 < nt) {
-            rowoff[(slot ^ 1) * 128 + t] = off;
-            bar_sync(2, 128);
-            if (tile + 1 < g.ct) fetch(cur, A.c.k, slot ^ 1);
-          }
-          wait_empty(vempty(st), ephase);
-          widen_store(nxt, vdst);
-          fence_proxy_async_smem();
-          mbar_arrive(vfull(st));
-        } else {
-          wait_empty(kempty(st), ephase);
-          node_rows((const bf16*)A.a.k, A.a.k_row, A.a.k_head, tile, kdst, false);
-          fence_proxy_async_smem();
-          mbar_arrive(kfull(st));
-          wait_empty(vempty(st), ephase);
-          if (t < MAX_NODES / 32 && tile == max(g.ct, g.t0)) odd[seg & 3][t] = 0u;
-          bar_sync(2, 128);
-          node_rows((const bf16*)A.a.v, A.a.v_row, A.a.v_head, tile, vdst, true);
-          fence_proxy_async_smem();
-          mbar_arrive(vfull(st));
-          off = -1; ks = vs = 1.f;
-          if (CODE != PCPB_BF16 && i + 1 < nt) { rowoff[(slot ^ 1) * 128 + t] = off; bar_sync(2, 128); }
+      for (int i = 0; i < nt; ++i, ++gi) {
+        const int tile = g.t0 + i, st = gi & 1, in = gi % INFO;
+        const bool cached = tile < g.ct;
+        if (!vals) {                                            // description of the tile
+          wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
+          float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
+          info[t] = f0.ks * (A.a.scale * LOG2E); info[128 + t] = f0.vs;
+          const uint32_t valid = __ballot_sync(0xffffffffu, f0.off >= 0);
+          if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
+          mbar_arrive(ifull(in));
         }
+        // the next tile's rows, and the pages of the one after
+        if (i + 1 < nt) { rowoff[(st ^ 1) * 128 + t] = f1.off; }
+        bar_sync(bar, 128);
+        const uint32_t dst = dst0 + st * Cfg::TILE_BYTES, full = full0 + 8u * st;
+        wait_empty(empty0 + 8u * st, ((gi >> 1) & 1) ^ 1);
+        if (CODE == PCPB_BF16 && cached) {
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+            const long long o = rowoff[st * 128 + row];
+            cp_async16z(dst + sw_off(row, c), pages + (o < 0 ? 0 : o + c * 16), o >= 0);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (pending) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            fence_proxy_async_smem();
+            mbar_arrive(pending);
+          }
+          pending = full;
+        } else if (cached) {
+          const bool more = i + 1 < nt && tile + 1 < g.ct;
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
+            uint32_t p[8];
+            constexpr int CC = CODE == PCPB_BF16 ? PCPB_I8 : CODE;
+            const uint4 r = cur[CODE == PCPB_BF16 ? 0 : k];
+            widen4<CC>(r.x, p[0], p[1]); widen4<CC>(r.y, p[2], p[3]); widen4<CC>(r.z, p[4], p[5]); widen4<CC>(r.w, p[6], p[7]);
+            if (more) cur[CODE == PCPB_BF16 ? 0 : k] = piece(k, st ^ 1);
+            const int flip = (c >> 2) & 1;                      // pieces of the second half go the other way round: other banks than the first half's
+            st_shared16(dst + sw_off(row, 2 * c + flip), p[flip ? 4 : 0], p[flip ? 5 : 1], p[flip ? 6 : 2], p[flip ? 7 : 3]);
+            st_shared16(dst + sw_off(row, 2 * c + 1 - flip), p[flip ? 0 : 4], p[flip ? 1 : 5], p[flip ? 2 : 6], p[flip ? 3 : 7]);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(full);
+        } else {
+          // rows of the nodes (bf16); values that are not numbers are left out and their nodes marked
+          const int n0 = (tile - g.ct) * TILE;
+          flush();
+          if (vals && tile == max(g.ct, g.t0)) {
+            if (t < MAX_NODES / 32) odd[seg & 3][t] = 0u;
+            bar_sync(bar, 128);
+          }
+#pragma unroll 1
+          for (int base = 0; base < PB; base += 8) {            // eight pieces in flight
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int idx = t + 128 * (base + k), node = n0 + idx / PB;
+              v[k] = make_uint4(0u, 0u, 0u, 0u);
+              if (node < g.s.n) v[k] = *reinterpret_cast<const uint4*>(nodes + (long long)(g.s.n0 + node) * node_row + (long long)g.kvh * node_head + idx % PB * 8);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int idx = t + 128 * (base + k), row = idx / PB, node = n0 + row;
+              uint32_t q[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+              if (vals) {
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  if ((q[j] & 0x7F80u) == 0x7F80u) { q[j] &= 0xFFFF0000u; bad = true; }
+                  if ((q[j] & 0x7F800000u) == 0x7F800000u) { q[j] &= 0x0000FFFFu; bad = true; }
+                }
+                if (bad) atomicOr(&odd[seg & 3][(node >> 5) & 7], 1u << (node & 31));
+              }
+              st_shared16(dst + sw_off(row, idx % PB), q[0], q[1], q[2], q[3]);
+            }
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(full);
+        }
+        f0 = f1; f1 = find(e2); e2 = look(tile + 3);
       }
       w += nt;
     }
     flush();
-  } else if (warp == 12) {
-    // =========================== MMA issuer ===========================
-    constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-    constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-    int gi = 0, seg = 0;
-    int pv[2] = {0, 0};                                         // output products of a stream so far
-    for (long long w = w0; w < w1; ++seg) {
-      const Seg g = seg_at(A, plan, w, w1);
-      const int nt = g.t1 - g.t0;
-      const bool pair = g.rows > 128;
-      const int cnt[2] = {pair ? nt : (nt + 1) / 2, pair ? nt : nt / 2};
-      wait(qfull, seg & 1, &fail);
-      tc_fence_after();
-      auto qk = [&](int x, int j) {
-        const int i = gi + (pair ? j : 2 * j + x), st = i & 1;
-        wait(kfull(st), (i >> 1) & 1, &fail);
-        tc_fence_after();
-        const uint32_t a = sQ + (pair ? x * Cfg::TILE_BYTES : 0), b = sK + st * Cfg::TILE_BYTES;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t o = (uint32_t)(k >> 2) * 16384u + (uint32_t)(k & 3) * 32u;
-          mma_bf16_elect(s_col(x), make_desc(a + o, 16, 1024), make_desc(b + o, 16, 1024), ID_S, k > 0);
-        }
-        mma_commit_elect(sfull(x));
-        if (!pair || x == 1) mma_commit_elect(kempty(st));
-      };
-      if (cnt[0] > 0) qk(0, 0);
-      if (cnt[1] > 0) qk(1, 0);
-      for (int j = 0; j < cnt[0]; ++j) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (j >= cnt[x]) continue;
-          const int i = gi + (pair ? j : 2 * j + x), st = i & 1;
-          wait(pfull(x), pv[x] & 1, &fail);
-          wait(vfull(st), (i >> 1) & 1, &fail);
-          if (j == 0) wait(oempty(x), (seg & 1) ^ 1, &fail);    // the last segment's output has been read
-          tc_fence_after();
-          const uint32_t b = sV + st * Cfg::TILE_BYTES;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_bf16_ts_elect(o_col(x), s_col(x) + 8u * k, make_desc(b + k * 2048u, 16384, 1024), ID_O, j > 0 || k > 0);
-          mma_commit_elect(pvdone(x));
-          if (!pair || x == 1) mma_commit_elect(vempty(st));
-          ++pv[x];
-          if (j + 1 < cnt[x]) qk(x, j + 1);
-        }
-      }
-      mma_commit_elect(odone);
-      gi += nt;
-      w += nt;
-    }
   } else {
     // =========================== softmax ===========================
     const int x = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     const float zscale = A.a.scale * LOG2E;
+    constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    const bool issuer = q4 == 0;
     int gi = 0, seg = 0, sn = 0;                                // tiles, segments; score tiles of this stream so far
     int16_t* par = reinterpret_cast<int16_t*>(gen + Cfg::OFF_PAR);
     float* ml = reinterpret_cast<float*>(gen + Cfg::OFF_ML);
@@ -845,6 +806,38 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         fence_proxy_async_smem();
         mbar_arrive(qfull);
       }
+      // products of tile i of the segment; a ring place is free when both streams' products (one stream: its own, twice) are done
+      auto issue_qk = [&](int i) {
+        const int at = gi + i, st = at & 1;
+        wait(kfull(st), (at >> 1) & 1, &fail);
+        tc_fence_after();
+        const uint32_t a = sQ + (pair ? x * Cfg::TILE_BYTES : 0), b = sK + st * Cfg::TILE_BYTES;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t o = (uint32_t)(k >> 2) * 16384u + (uint32_t)(k & 3) * 32u;
+          mma_bf16_elect(s_col(x), make_desc(a + o, 16, 1024), make_desc(b + o, 16, 1024), ID_S, k > 0);
+        }
+        mma_commit_elect(sfull(x));
+        mma_commit_elect(kempty(st));
+        if (!pair) mma_commit_elect(kempty(st));
+      };
+      auto issue_pv = [&](int i, bool first) {
+        const int at = gi + i, st = at & 1;
+        wait(vfull(st), (at >> 1) & 1, &fail);
+        tc_fence_after();
+        const uint32_t b = sV + st * Cfg::TILE_BYTES;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_bf16_ts_elect(o_col(x), s_col(x) + 8u * k, make_desc(b + k * 2048u, 16384, 1024), ID_O, !first || k > 0);
+        mma_commit_elect(pvdone(x));
+        mma_commit_elect(vempty(st));
+        if (!pair) mma_commit_elect(vempty(st));
+      };
+      const int step = pair ? 1 : 2;
+      if (issuer) {
+        wait(qfull, seg & 1, &fail);
+        if ((pair ? 0 : x) < nt) issue_qk(pair ? 0 : x);
+      }
       const bool has_tree = g.t1 > g.ct;
       uint32_t anc[MAX_NODES / 32] = {};
       if (has_tree) {
@@ -863,7 +856,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       }
       float mref = -INFINITY, l = 0.f;
       int done = 0;                                             // tiles of this stream in this segment
-      for (int i = pair ? 0 : x; i < nt; i += pair ? 1 : 2, ++done, ++sn) {
+      for (int i = pair ? 0 : x; i < nt; i += step, ++done, ++sn) {
         const int in = (gi + i) % INFO;
         wait(ifull(in), ((gi + i) / INFO) & 1, &fail);
         wait(sfull(x), sn & 1, &fail);
@@ -884,24 +877,37 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           const bool all = __all_sync(0xffffffffu, (see[0] & see[1] & see[2] & see[3]) == 0xffffffffu && own < 0);
           // largest score
           float mx = -INFINITY;
+          if (all) {
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t v[2][16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(s_col(x) + lane_off + 32u * c, v);
-            if (all) {
+              for (int h = 0; h < 2; ++h) tmem_ld16_issue(s_col(x) + lane_off + c + 16u * h, v[h]);
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                float f[4] = {1.f, 1.f, 1.f, 1.f};
-                if (CODE != PCPB_BF16) { const float4 k4 = *reinterpret_cast<const float4*>(info + 32 * c + j); f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w; }
+              for (int h = 0; h < 2; ++h) {
+                tmem_ld_wait16(v[h]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, __uint_as_float(v[j + k]) * (zscale * f[k]));
+                for (int j = 0; j < 16; j += 4) {
+                  float f[4] = {zscale, zscale, zscale, zscale};
+                  if (CODE != PCPB_BF16) { const float4 k4 = *reinterpret_cast<const float4*>(info + c + 16 * h + j); f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w; }
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], __uint_as_float(v[h][j + k]) * f[k]);
+                }
               }
-            } else {
+            }
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t word = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
+              uint32_t v[32];
+              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                float z = __uint_as_float(v[j]) * (zscale * info[32 * c + j]);
+                float z = __uint_as_float(v[j]) * info[32 * c + j];
                 if (32 * c + j == own) z = 0.f;
-                if ((see[c] >> j) & 1u) mx = fmaxf(mx, z);
+                if ((word >> j) & 1u) mx = fmaxf(mx, z);
               }
             }
           }
@@ -932,39 +938,54 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           }
           const float ref = mref == -INFINITY ? 0.f : mref;
           // weights
+          if (all) {
+            float l4[4] = {l, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t v[2][16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], p[16];
-            tmem_ld32(s_col(x) + lane_off + 32u * c, v);
-            if (all) {
+              for (int h = 0; h < 2; ++h) tmem_ld16_issue(s_col(x) + lane_off + c + 16u * h, v[h]);
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                float f[4] = {1.f, 1.f, 1.f, 1.f}, h[4] = {1.f, 1.f, 1.f, 1.f}, e[4];
-                if (CODE != PCPB_BF16) {
-                  const float4 k4 = *reinterpret_cast<const float4*>(info + 32 * c + j), v4 = *reinterpret_cast<const float4*>(info + 128 + 32 * c + j);
-                  f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w;
-                  h[0] = v4.x; h[1] = v4.y; h[2] = v4.z; h[3] = v4.w;
+              for (int h = 0; h < 2; ++h) {
+                uint32_t p[8];
+                tmem_ld_wait16(v[h]);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  float f[4] = {zscale, zscale, zscale, zscale}, y[4] = {1.f, 1.f, 1.f, 1.f}, e[4];
+                  if (CODE != PCPB_BF16) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(info + c + 16 * h + j), v4 = *reinterpret_cast<const float4*>(info + 128 + c + 16 * h + j);
+                    f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w;
+                    y[0] = v4.x; y[1] = v4.y; y[2] = v4.z; y[3] = v4.w;
+                  }
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    e[k] = ex2(fmaf(__uint_as_float(v[h][j + k]), f[k], -ref));
+                    l4[k] += e[k];
+                    if (CODE != PCPB_BF16) e[k] *= y[k];
+                  }
+                  p[j / 2] = pack2(e[0], e[1]); p[j / 2 + 1] = pack2(e[2], e[3]);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  e[k] = ex2(fmaf(__uint_as_float(v[j + k]), zscale * f[k], -ref));
-                  l += e[k];
-                  if (CODE != PCPB_BF16) e[k] *= h[k];
-                }
-                p[j / 2] = pack2(e[0], e[1]); p[j / 2 + 1] = pack2(e[2], e[3]);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float z = __uint_as_float(v[j]) * (zscale * info[32 * c + j]);
-                if (32 * c + j == own) z = 0.f;
-                float e = (see[c] >> j) & 1u ? ex2(z - ref) : 0.f;
-                l += e;
-                e = (see[c] >> j) & 1u && 32 * c + j != own ? e * info[128 + 32 * c + j] : 0.f;
-                if (j & 1) p[j / 2] = pack2(__uint_as_float(p[j / 2]), e); else p[j / 2] = __float_as_uint(e);
+                tmem_st8(s_col(x) + lane_off + c / 2 + 8u * h, p);
               }
             }
-            tmem_st16(s_col(x) + lane_off + 16u * c, p);
+            l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t word = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
+              uint32_t v[32], p[16];
+              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float z = __uint_as_float(v[j]) * info[32 * c + j];
+                if (32 * c + j == own) z = 0.f;
+                float e = (word >> j) & 1u ? ex2(z - ref) : 0.f;
+                l += e;
+                e = (word >> j) & 1u && 32 * c + j != own ? e * info[128 + 32 * c + j] : 0.f;
+                if (j & 1) p[j / 2] = pack2(__uint_as_float(p[j / 2]), e); else p[j / 2] = __float_as_uint(e);
+              }
+              tmem_st16(s_col(x) + lane_off + 16u * c, p);
+            }
           }
           tmem_st_wait();
         }
@@ -974,7 +995,14 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           mbar_arrive(pfull(x));
           mbar_arrive_n(iempty(in), pair ? 1u : 2u);
         }
+        if (issuer) {
+          wait(pfull(x), sn & 1, &fail);
+          tc_fence_after();
+          issue_pv(i, done == 0);
+          if (i + step < nt) issue_qk(i + step);
+        }
       }
+      if (issuer) mma_commit_elect(odone);
       // the segment's end: outputs of both streams are complete
       wait(odone, seg & 1, &fail);
       tc_fence_after();
@@ -1047,8 +1075,8 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) { mbar_arrive(oempty(0)); mbar_arrive(oempty(1)); }
-      bar_sync(1, 256);                                         // ml, par and q are used again
+      bar_sync(1, 256);                                         // the outputs, ml, par and q are used again
+      tc_fence_after();
       gi += nt;
       w += nt;
     }
@@ -1057,7 +1085,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && fail) op_note(A.status, PCPB_OPS_STUCK);
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------

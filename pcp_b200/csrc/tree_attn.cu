@@ -40,25 +40,37 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Pairs of f32 in one 64-bit register: one instruction for both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk2(float a, float b) { f32x2 d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ void un2(f32x2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t bsub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 // Four codes in a word -> two pairs of bf16 (exact: both code types have fewer significant bits than bf16).
 //   e4m3: sign and the seven other bits move to the bf16 fields of the same name; the exponent's bias then differs by
 //         127 - 7 = 120, which one product with 2^120 repairs, for subnormal codes as well.
-//   i8:   the code plus 128 in the low byte of 2^23's bit pattern is the float 2^23 + 128 + code.
+//   i8:   with c7 the sign bit and c the other seven, 0x4300 + c is 128 + c and 0x4300 + (c7 << 7) is 128 or 256; the code is their difference.
 template <int CODE> __device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
   if (CODE == PCPB_E4M3) {
     const uint32_t t0 = __byte_perm(w, 0, 0x1404), t1 = __byte_perm(w, 0, 0x3424);
     p01 = bmul2(((t0 >> 4) & 0x07F007F0u) | (t0 & 0x80008000u), 0x7B807B80u);
     p23 = bmul2(((t1 >> 4) & 0x07F007F0u) | (t1 & 0x80008000u), 0x7B807B80u);
   } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const float k = 8388608.f + 128.f;
-    p01 = pack2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650)) - k, __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7651)) - k);
-    p23 = pack2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7652)) - k, __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7653)) - k);
+    const uint32_t t0 = __byte_perm(w, 0, 0x4140), t1 = __byte_perm(w, 0, 0x4342);
+    p01 = bsub2((t0 & 0x007F007Fu) | 0x43004300u, (t0 & 0x00800080u) | 0x43004300u);
+    p23 = bsub2((t1 & 0x007F007Fu) | 0x43004300u, (t1 & 0x00800080u) | 0x43004300u);
   }
 }
 
@@ -527,11 +539,12 @@ constexpr int INFO = 4;              // tile descriptions in flight
 template <int HD> struct TcCfg {
   static constexpr int TILE_BYTES = 128 * HD * 2;
   static constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + 2 * TILE_BYTES, OFF_INFO = OFF_V + 2 * TILE_BYTES;
-  static constexpr int INFO_BYTES = 2 * 128 * 4 + 16;                     // key scales, value scales, valid positions
+  static constexpr int INFO_BYTES = 2 * 128 * 4 + 16;                     // key scales, value scales, valid positions (a word for 32)
   static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2 loader groups][2][128] byte offsets of rows
   static constexpr int OFF_ML = OFF_ROW + 4 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
   static constexpr int OFF_PAR = OFF_ML + 2 * 128 * 2 * 4;                // parents
-  static constexpr int OFF_BAR = OFF_PAR + MAX_NODES * 2;
+  static constexpr int OFF_ANC = OFF_PAR + MAX_NODES * 2;                 // [MAX_NODES / 32][256] ancestors-or-self of the rows' nodes
+  static constexpr int OFF_BAR = OFF_ANC + MAX_NODES / 32 * 256 * 4;
   static constexpr int OFF_PLAN = OFF_BAR + 256;
   static constexpr int BYTES = OFF_PLAN + (MAX_BATCH + 1) * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory");
@@ -696,7 +709,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         if (!vals) {                                            // description of the tile
           wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
           float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
-          info[t] = f0.ks * (A.a.scale * LOG2E); info[128 + t] = f0.vs;
+          info[t] = f0.ks * (fabsf(A.a.scale) * LOG2E); info[128 + t] = f0.vs;
           const uint32_t valid = __ballot_sync(0xffffffffu, f0.off >= 0);
           if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
           mbar_arrive(ifull(in));
@@ -781,13 +794,15 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     // =========================== softmax ===========================
     const int x = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-    const float zscale = A.a.scale * LOG2E;
+    const float zscale = fabsf(A.a.scale) * LOG2E;             // a negative scale changes the sign of q instead
+    const uint32_t qsign = A.a.scale < 0.f ? 0x80008000u : 0u;
     constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     const bool issuer = q4 == 0;
     int gi = 0, seg = 0, sn = 0;                                // tiles, segments; score tiles of this stream so far
     int16_t* par = reinterpret_cast<int16_t*>(gen + Cfg::OFF_PAR);
     float* ml = reinterpret_cast<float*>(gen + Cfg::OFF_ML);
+    uint32_t* anc = reinterpret_cast<uint32_t*>(gen + Cfg::OFF_ANC) + threadIdx.x;       // this thread's row: word k at anc[256 k]
     for (long long w = w0; w < w1; ++seg) {
       const Seg g = seg_at(A, plan, w, w1);
       const int nt = g.t1 - g.t0;
@@ -801,7 +816,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         const int c0 = pair ? 0 : x * (HD / 16), c1 = pair ? HD / 8 : c0 + HD / 16;
         for (int c = c0; c < c1; ++c) {
           const uint4 v = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-          st_shared16(dst + sw_off(r, c), v.x, v.y, v.z, v.w);
+          st_shared16(dst + sw_off(r, c), v.x ^ qsign, v.y ^ qsign, v.z ^ qsign, v.w ^ qsign);
         }
         fence_proxy_async_smem();
         mbar_arrive(qfull);
@@ -839,7 +854,6 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         if ((pair ? 0 : x) < nt) issue_qk(pair ? 0 : x);
       }
       const bool has_tree = g.t1 > g.ct;
-      uint32_t anc[MAX_NODES / 32] = {};
       if (has_tree) {
         for (int i = threadIdx.x; i < g.s.n; i += 256) {
           int bad = 0;
@@ -847,143 +861,142 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
         }
         bar_sync(1, 256);
-        int i = live ? node : -1;
-        while (i >= 0) {
-#pragma unroll
-          for (int k = 0; k < MAX_NODES / 32; ++k) anc[k] |= (i >> 5) == k ? 1u << (i & 31) : 0u;
-          i = par[i];
-        }
+#pragma unroll 1
+        for (int k = 0; k < MAX_NODES / 32; ++k) anc[256 * k] = 0u;
+#pragma unroll 1
+        for (int i = live ? node : -1; i >= 0; i = par[i]) anc[256 * (i >> 5)] |= 1u << (i & 31);
       }
-      float mref = -INFINITY, l = 0.f;
+      float mref = -INFINITY;
+      f32x2 l2 = pk2(0.f, 0.f);
       int done = 0;                                             // tiles of this stream in this segment
       for (int i = pair ? 0 : x; i < nt; i += step, ++done, ++sn) {
         const int in = (gi + i) % INFO;
+        const float* info = reinterpret_cast<const float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
+        const int tile = g.t0 + i;
+        const bool tree = tile >= g.ct;
         wait(ifull(in), ((gi + i) / INFO) & 1, &fail);
+        const uint4 valid = *reinterpret_cast<const uint4*>(info + 256);
+        const bool all = !tree && (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
         wait(sfull(x), sn & 1, &fail);
         tc_fence_after();
         if (warp_live) {
-          const float* info = reinterpret_cast<const float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
-          const int tile = g.t0 + i;
-          const bool tree = tile >= g.ct;
-          uint32_t see[4];
-          if (tree) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) see[k] = tile == g.ct ? anc[k] : anc[4 + k];
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) see[k] = reinterpret_cast<const uint32_t*>(info)[256 + k];
-          }
-          const int own = tree && A.a.null_self ? node - (tile - g.ct) * TILE : -1;
-          const bool all = __all_sync(0xffffffffu, (see[0] & see[1] & see[2] & see[3]) == 0xffffffffu && own < 0);
-          // largest score
-          float mx = -INFINITY;
-          if (all) {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              uint32_t v[2][16];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) tmem_ld16_issue(s_col(x) + lane_off + c + 16u * h, v[h]);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                tmem_ld_wait16(v[h]);
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  float f[4] = {zscale, zscale, zscale, zscale};
-                  if (CODE != PCPB_BF16) { const float4 k4 = *reinterpret_cast<const float4*>(info + c + 16 * h + j); f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w; }
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], __uint_as_float(v[h][j + k]) * f[k]);
-                }
-              }
-            }
-            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t word = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
-              uint32_t v[32];
-              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float z = __uint_as_float(v[j]) * info[32 * c + j];
-                if (32 * c + j == own) z = 0.f;
-                if ((word >> j) & 1u) mx = fmaxf(mx, z);
-              }
-            }
-          }
-          // move the reference maximum
-          const bool up = mx > mref + 8.f || (mref == -INFINITY && mx > -INFINITY);
-          if (__any_sync(0xffffffffu, up)) {
-            const float ref = up ? mx : mref;
-            const float corr = up && mref > -INFINITY ? ex2(mref - ref) : 1.f;
+          // The reference maximum moves (rarely): outputs, sums and the tile's weights so far (columns below 32 c) are scaled down.
+          auto raise = [&](float top, int c) {
+            const bool up = top > mref + 8.f || (mref == -INFINITY && top > -INFINITY);
+            const float to = up ? top : mref, corr = up && mref > -INFINITY ? ex2(mref - to) : 1.f;
             if (done > 0) {
               wait(pvdone(x), (sn - 1) & 1, &fail);
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld32(o_col(x) + lane_off + 32u * c, v);
+              for (int k = 0; k < HD; k += 16) {
+                uint32_t u[16];
+                tmem_ld16(o_col(x) + lane_off + k, u);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  uint32_t u[16];
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(v[16 * h + j]) * corr);
-                  tmem_st16(o_col(x) + lane_off + 32u * c + 16u * h, u);
-                }
+                for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * corr);
+                tmem_st16(o_col(x) + lane_off + k, u);
               }
-              tmem_st_wait();
             }
-            l *= corr;
-            mref = ref;
-          }
-          const float ref = mref == -INFINITY ? 0.f : mref;
-          // weights
-          if (all) {
-            float l4[4] = {l, 0.f, 0.f, 0.f};
 #pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              uint32_t v[2][16];
+            for (int k = 0; k < c; ++k) {
+              uint32_t u[16];
+              tmem_ld16(s_col(x) + lane_off + 16u * k, u);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) tmem_ld16_issue(s_col(x) + lane_off + c + 16u * h, v[h]);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t p[8];
-                tmem_ld_wait16(v[h]);
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  float f[4] = {zscale, zscale, zscale, zscale}, y[4] = {1.f, 1.f, 1.f, 1.f}, e[4];
-                  if (CODE != PCPB_BF16) {
-                    const float4 k4 = *reinterpret_cast<const float4*>(info + c + 16 * h + j), v4 = *reinterpret_cast<const float4*>(info + 128 + c + 16 * h + j);
-                    f[0] = k4.x; f[1] = k4.y; f[2] = k4.z; f[3] = k4.w;
-                    y[0] = v4.x; y[1] = v4.y; y[2] = v4.z; y[3] = v4.w;
-                  }
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    e[k] = ex2(fmaf(__uint_as_float(v[h][j + k]), f[k], -ref));
-                    l4[k] += e[k];
-                    if (CODE != PCPB_BF16) e[k] *= y[k];
-                  }
-                  p[j / 2] = pack2(e[0], e[1]); p[j / 2 + 1] = pack2(e[2], e[3]);
-                }
-                tmem_st8(s_col(x) + lane_off + c / 2 + 8u * h, p);
-              }
+              for (int j = 0; j < 16; ++j) u[j] = pack2(bf_lo(u[j]) * corr, bf_hi(u[j]) * corr);
+              tmem_st16(s_col(x) + lane_off + 16u * k, u);
             }
-            l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            tmem_st_wait();
+            l2 = mul2(l2, pk2(corr, corr));
+            mref = to;
+          };
+          if (all) {
+            // 32 columns at a time.  The weights are formed with the
+            // reference maximum as it stands, and once more in the rare case that it has to move.
+            auto chunk = [&](uint32_t (&v)[32], int c) {
+              float z[32], top;
+              uint32_t p[16];
+              f32x2 sum;
+              const ulonglong2* k4 = reinterpret_cast<const ulonglong2*>(info + 32 * c);
+              const ulonglong2* v4 = reinterpret_cast<const ulonglong2*>(info + 128 + 32 * c);
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                if (CODE != PCPB_BF16) {
+                  const ulonglong2 f = k4[j / 4];
+                  un2(mul2(pk2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f.x), z[j], z[j + 1]);
+                  un2(mul2(pk2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), f.y), z[j + 2], z[j + 3]);
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) z[j + k] = __uint_as_float(v[j + k]);
+                }
+              }
+              for (;;) {
+                const float ref = mref == -INFINITY ? 0.f : mref;
+                const f32x2 nref = pk2(-ref, -ref), zs = pk2(zscale, zscale);
+                f32x2 s0 = pk2(0.f, 0.f), s1 = s0;
+                float m0 = z[0], m1 = z[1];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                  f32x2 d0 = pk2(z[j], z[j + 1]), d1 = pk2(z[j + 2], z[j + 3]);
+                  d0 = CODE == PCPB_BF16 ? fma2(d0, zs, nref) : add2(d0, nref);
+                  d1 = CODE == PCPB_BF16 ? fma2(d1, zs, nref) : add2(d1, nref);
+                  float e0, e1, e2, e3;
+                  un2(d0, e0, e1); un2(d1, e2, e3);
+                  m0 = max3(m0, z[j], z[j + 1]); m1 = max3(m1, z[j + 2], z[j + 3]);
+                  e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
+                  d0 = pk2(e0, e1); d1 = pk2(e2, e3);
+                  s0 = add2(s0, d0); s1 = add2(s1, d1);
+                  if (CODE != PCPB_BF16) {
+                    const ulonglong2 y = v4[j / 4];
+                    un2(mul2(d0, y.x), e0, e1); un2(mul2(d1, y.y), e2, e3);
+                  }
+                  p[j / 2] = pack2(e0, e1); p[j / 2 + 1] = pack2(e2, e3);
+                }
+                top = fmaxf(m0, m1);
+                if (CODE == PCPB_BF16) top *= zscale;
+                sum = add2(s0, s1);
+                if (!__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) break;
+                raise(top, c);
+              }
+              l2 = add2(l2, sum);
+              tmem_st16(s_col(x) + lane_off + 16u * c, p);
+            };
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+              chunk(v, c);
+            }
           } else {
+            uint32_t see[4] = {valid.x, valid.y, valid.z, valid.w};
+            if (tree) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) see[k] = anc[256 * ((tile - g.ct) * (TILE / 32) + k)];
+            }
+            const int own = tree && A.a.null_self ? node - (tile - g.ct) * TILE : -1;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               const uint32_t word = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
               uint32_t v[32], p[16];
               tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+              float top = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 float z = __uint_as_float(v[j]) * info[32 * c + j];
                 if (32 * c + j == own) z = 0.f;
-                float e = (word >> j) & 1u ? ex2(z - ref) : 0.f;
-                l += e;
-                e = (word >> j) & 1u && 32 * c + j != own ? e * info[128 + 32 * c + j] : 0.f;
+                z = (word >> j) & 1u ? z : -INFINITY;
+                top = fmaxf(top, z);
+                v[j] = __float_as_uint(z);
+              }
+              if (__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) raise(top, c);
+              const float ref = mref == -INFINITY ? 0.f : mref;
+              float add = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float e = ex2(__uint_as_float(v[j]) - ref);     // a masked column's weight is 0
+                add += e;
+                e = 32 * c + j != own && (word >> j) & 1u ? e * info[128 + 32 * c + j] : 0.f;
                 if (j & 1) p[j / 2] = pack2(__uint_as_float(p[j / 2]), e); else p[j / 2] = __float_as_uint(e);
               }
+              l2 = add2(l2, pk2(add, 0.f));
               tmem_st16(s_col(x) + lane_off + 16u * c, p);
             }
           }
@@ -1003,6 +1016,9 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         }
       }
       if (issuer) mma_commit_elect(odone);
+      float l, lo;
+      un2(l2, l, lo);
+      l += lo;
       // the segment's end: outputs of both streams are complete
       wait(odone, seg & 1, &fail);
       tc_fence_after();
@@ -1028,8 +1044,8 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         float* part = A.part_o + (slot * TR + tr) * HD;
         bool strange = false;
         if (has_tree) {
-#pragma unroll
-          for (int k = 0; k < MAX_NODES / 32; ++k) strange |= (anc[k] & odd[seg & 3][k]) != 0u;
+#pragma unroll 1
+          for (int k = 0; k < MAX_NODES / 32; ++k) strange |= (anc[256 * k] & odd[seg & 3][k]) != 0u;
         }
         // columns: with two row tiles all of the row's; else the warps of the two groups take half of them each
         const int c0 = pair ? 0 : x * (HD / 32), c1 = pair ? HD / 16 : c0 + HD / 32;
@@ -1049,10 +1065,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           }
           if (strange)                                          // infinities and NaN of the values this row does attend
             for (int i = max(0, g.t0 - g.ct) * TILE; i < min(g.s.n, (g.t1 - g.ct) * TILE); ++i) {
-              uint32_t word = 0;
-#pragma unroll
-              for (int k = 0; k < MAX_NODES / 32; ++k) word = (i >> 5) == k ? anc[k] & odd[seg & 3][k] : word;
-              if (!((word >> (i & 31)) & 1u) || (A.a.null_self && i == node)) continue;
+              if (!(((anc[256 * (i >> 5)] & odd[seg & 3][i >> 5]) >> (i & 31)) & 1u) || (A.a.null_self && i == node)) continue;
               const bf16* vr = (const bf16*)A.a.v + (long long)(g.s.n0 + i) * A.a.v_row + (long long)g.kvh * A.a.v_head + 16 * c;
 #pragma unroll
               for (int j = 0; j < 16; ++j) { const float y = to_f(vr[j]); if (!isfinite(y)) o[j] += y; }

@@ -315,6 +315,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_t
   __shared__ int16_t par[MAX_NODES];
   __shared__ uint32_t anc[RW][MAX_NODES / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;");
   make_plan<RW>(A, plan);
   const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
   if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
@@ -481,7 +482,12 @@ template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_t
   }
 }
 
-// Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles, ROWS / 16): a block joins 16 rows.
+// Programmatic dependent launch: the join's blocks may be set up while the attention kernel drains; they wait for its results themselves.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles, ROWS / 16): a block joins 16 rows, a thread
+// four columns of one or more of them.
 template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ AttnArgs A, int blocks) {
   const int b = blockIdx.x;
   const Seq s = seq_of(A, b);
@@ -490,21 +496,36 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
   if (item >= RT * A.c.n_kv_head) return;
   const int kvh = item / RT, row0 = item % RT * ROWS, r0 = blockIdx.z * 16;
   if (row0 + r0 >= rows) return;
+  pdl_wait();
   const Parts P = parts_of(A.plan[b] + (long long)item * T, T, tile_share(A.plan[A.c.batch], blocks));
   if (P.c0 == P.c1) return;
   for (int i = threadIdx.x; i < 16 * (HD / 4); i += blockDim.x) {
     const int r = r0 + i / (HD / 4), c = i % (HD / 4) * 4;
     if (row0 + r >= rows) continue;
-    float m = -INFINITY;
-    for (int k = P.c0; k <= P.c1; ++k) m = fmaxf(m, A.part_ml[((size_t)part_slot(P, k) * ROWS + r) * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[4] = {};
-    for (int k = P.c0; k <= P.c1; ++k) {
-      const size_t at = (size_t)part_slot(P, k) * ROWS + r;
-      const float f = ex2(A.part_ml[at * 2] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(A.part_o + at * HD + c);
-      l += f * A.part_ml[at * 2 + 1];
-      o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
+    float m = -INFINITY, l = 0.f, o[4] = {};
+    for (int k0 = P.c0; k0 <= P.c1; k0 += 4) {                  // four parts in flight, taken in block order
+      float2 q[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        q[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k <= P.c1) {
+          const size_t at = (size_t)part_slot(P, k0 + k) * ROWS + r;
+          q[k] = *reinterpret_cast<const float2*>(A.part_ml + at * 2);
+          v[k] = *reinterpret_cast<const float4*>(A.part_o + at * HD + c);
+        }
+      }
+      const float top = fmaxf(fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), m), ref = top == -INFINITY ? 0.f : top;
+      const float f0 = ex2(m - ref);
+      m = top;
+      l *= f0; o[0] *= f0; o[1] *= f0; o[2] *= f0; o[3] *= f0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ex2(q[k].x - ref);
+        l += f * q[k].y;
+        o[0] += f * v[k].x; o[1] += f * v[k].y; o[2] += f * v[k].z; o[3] += f * v[k].w;
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int node = (row0 + r) / A.G, h = kvh * A.G + (row0 + r) % A.G;
@@ -575,10 +596,11 @@ __device__ __forceinline__ Seg seg_at(const AttnArgs& A, const long long* plan, 
   g.s = seq_of(A, g.b);
   g.ct = tiles_of(g.s.ctx); g.T = g.ct + tiles_of(g.s.n);
   const int all = g.s.n * A.G, RT = (all + TR - 1) / TR;
-  const long long at = w - plan[g.b], item = at / g.T;
-  g.t0 = (int)(at % g.T);
+  const long long at = w - plan[g.b];
+  const long long item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)g.T) : at / g.T;
+  g.t0 = (int)(at - item * g.T);
   g.t1 = (int)min((long long)g.T, g.t0 + (w1 - w));
-  g.kvh = (int)(item / RT); g.row0 = (int)(item % RT) * TR;
+  g.kvh = (int)item / RT; g.row0 = ((int)item - g.kvh * RT) * TR;          // items of a sequence: kv heads x row tiles, an int
   g.rows = min(TR, all - g.row0);
   return g;
 }
@@ -604,6 +626,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
   const uint32_t qfull = sBar + 192u, odone = sBar + 200u;
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
+  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     fail = 0;
     for (int i = 0; i < 2; ++i) {
@@ -709,7 +732,9 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         if (!vals) {                                            // description of the tile
           wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
           float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
-          info[t] = f0.ks * (fabsf(A.a.scale) * LOG2E); info[128 + t] = f0.vs;
+          const float factor = f0.ks * (fabsf(A.a.scale) * LOG2E);
+          info[t] = factor < 1.17549435e-38f ? 1.17549435e-38f : factor;           // (a NaN stays)
+          info[128 + t] = f0.vs;
           const uint32_t valid = __ballot_sync(0xffffffffu, f0.off >= 0);
           if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
           mbar_arrive(ifull(in));
@@ -794,7 +819,8 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     // =========================== softmax ===========================
     const int x = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-    const float zscale = fabsf(A.a.scale) * LOG2E;             // a negative scale changes the sign of q instead
+    // a negative scale changes the sign of q instead; a positive factor at least, so that a masked score stays -inf
+    const float zscale = fmaxf(fabsf(A.a.scale) * LOG2E, 1.17549435e-38f);
     const uint32_t qsign = A.a.scale < 0.f ? 0x80008000u : 0u;
     constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -810,13 +836,23 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       const int tr = pair ? x * 128 + r : r;                    // row of the item
       const bool live = tr < g.rows, warp_live = (pair ? x * 128 : 0) + q4 * 32 < g.rows;
       const int node = (g.row0 + tr) / A.G, head = g.kvh * A.G + (g.row0 + tr) % A.G;
+      const bool has_tree = g.t1 > g.ct;
+      if (has_tree && threadIdx.x < g.s.n) {                    // at most 256 nodes, as many threads
+        int bad = 0;
+        par[threadIdx.x] = (int16_t)clip_parent(A.a.parent ? A.a.parent[g.s.n0 + threadIdx.x] : (int)threadIdx.x - 1, threadIdx.x, &bad);
+        if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
+      }
       {
         const bf16* src = (const bf16*)A.a.q + (long long)(g.s.n0 + node) * A.a.q_row + (long long)head * A.a.q_head;
         const uint32_t dst = sQ + (pair ? x * Cfg::TILE_BYTES : 0);
         const int c0 = pair ? 0 : x * (HD / 16), c1 = pair ? HD / 8 : c0 + HD / 16;
-        for (int c = c0; c < c1; ++c) {
-          const uint4 v = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-          st_shared16(dst + sw_off(r, c), v.x ^ qsign, v.y ^ qsign, v.z ^ qsign, v.w ^ qsign);
+#pragma unroll 1
+        for (int c = c0; c < c1; c += HD / 16) {                // HD / 16 pieces in flight
+          uint4 v[HD / 16];
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) v[k] = live ? *reinterpret_cast<const uint4*>(src + (c + k) * 8) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) st_shared16(dst + sw_off(r, c + k), v[k].x ^ qsign, v[k].y ^ qsign, v[k].z ^ qsign, v[k].w ^ qsign);
         }
         fence_proxy_async_smem();
         mbar_arrive(qfull);
@@ -853,13 +889,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         wait(qfull, seg & 1, &fail);
         if ((pair ? 0 : x) < nt) issue_qk(pair ? 0 : x);
       }
-      const bool has_tree = g.t1 > g.ct;
       if (has_tree) {
-        for (int i = threadIdx.x; i < g.s.n; i += 256) {
-          int bad = 0;
-          par[i] = (int16_t)clip_parent(A.a.parent ? A.a.parent[g.s.n0 + i] : i - 1, i, &bad);
-          if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
-        }
         bar_sync(1, 256);
 #pragma unroll 1
         for (int k = 0; k < MAX_NODES / 32; ++k) anc[256 * k] = 0u;
@@ -876,7 +906,6 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         const bool tree = tile >= g.ct;
         wait(ifull(in), ((gi + i) / INFO) & 1, &fail);
         const uint4 valid = *reinterpret_cast<const uint4*>(info + 256);
-        const bool all = !tree && (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
         wait(sfull(x), sn & 1, &fail);
         tc_fence_after();
         if (warp_live) {
@@ -908,97 +937,72 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
             l2 = mul2(l2, pk2(corr, corr));
             mref = to;
           };
-          if (all) {
-            // 32 columns at a time.  The weights are formed with the
-            // reference maximum as it stands, and once more in the rare case that it has to move.
-            auto chunk = [&](uint32_t (&v)[32], int c) {
-              float z[32], top;
-              uint32_t p[16];
-              f32x2 sum;
-              const ulonglong2* k4 = reinterpret_cast<const ulonglong2*>(info + 32 * c);
-              const ulonglong2* v4 = reinterpret_cast<const ulonglong2*>(info + 128 + 32 * c);
+          // 32 columns at a time.  The weights are formed with the
+          // reference maximum as it stands, and once more in the rare case that it has to move.
+          auto chunk = [&](uint32_t (&v)[32], int c, int own) {
+            float z[32], top;
+            uint32_t p[16];
+            f32x2 sum;
+            const ulonglong2* k4 = reinterpret_cast<const ulonglong2*>(info + 32 * c);
+            const ulonglong2* v4 = reinterpret_cast<const ulonglong2*>(info + 128 + 32 * c);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              if (CODE != PCPB_BF16) {
+                const ulonglong2 f = k4[j / 4];
+                un2(mul2(pk2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f.x), z[j], z[j + 1]);
+                un2(mul2(pk2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), f.y), z[j + 2], z[j + 3]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[j + k] = __uint_as_float(v[j + k]);
+              }
+            }
+            for (;;) {
+              const float ref = mref == -INFINITY ? 0.f : mref;
+              const f32x2 nref = pk2(-ref, -ref), zs = pk2(zscale, zscale);
+              f32x2 s0 = pk2(0.f, 0.f), s1 = s0;
+              float m0 = z[0], m1 = z[1];
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
+                f32x2 d0 = pk2(z[j], z[j + 1]), d1 = pk2(z[j + 2], z[j + 3]);
+                d0 = CODE == PCPB_BF16 ? fma2(d0, zs, nref) : add2(d0, nref);
+                d1 = CODE == PCPB_BF16 ? fma2(d1, zs, nref) : add2(d1, nref);
+                float e0, e1, e2, e3;
+                un2(d0, e0, e1); un2(d1, e2, e3);
+                m0 = max3(m0, z[j], z[j + 1]); m1 = max3(m1, z[j + 2], z[j + 3]);
+                e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
+                d0 = pk2(e0, e1); d1 = pk2(e2, e3);
+                s0 = add2(s0, d0); s1 = add2(s1, d1);
                 if (CODE != PCPB_BF16) {
-                  const ulonglong2 f = k4[j / 4];
-                  un2(mul2(pk2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f.x), z[j], z[j + 1]);
-                  un2(mul2(pk2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), f.y), z[j + 2], z[j + 3]);
-                } else {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) z[j + k] = __uint_as_float(v[j + k]);
+                  const ulonglong2 y = v4[j / 4];
+                  un2(mul2(d0, y.x), e0, e1); un2(mul2(d1, y.y), e2, e3);
                 }
+                p[j / 2] = pack2(e0, e1); p[j / 2 + 1] = pack2(e2, e3);
               }
-              for (;;) {
-                const float ref = mref == -INFINITY ? 0.f : mref;
-                const f32x2 nref = pk2(-ref, -ref), zs = pk2(zscale, zscale);
-                f32x2 s0 = pk2(0.f, 0.f), s1 = s0;
-                float m0 = z[0], m1 = z[1];
+              top = fmaxf(m0, m1);
+              if (CODE == PCPB_BF16) top *= zscale;
+              sum = add2(s0, s1);
+              if (!__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) break;
+              raise(top, c);
+            }
+            l2 = add2(l2, sum);
+            if (own >= 0) {                                     // counted above, but its value is a zero
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                  f32x2 d0 = pk2(z[j], z[j + 1]), d1 = pk2(z[j + 2], z[j + 3]);
-                  d0 = CODE == PCPB_BF16 ? fma2(d0, zs, nref) : add2(d0, nref);
-                  d1 = CODE == PCPB_BF16 ? fma2(d1, zs, nref) : add2(d1, nref);
-                  float e0, e1, e2, e3;
-                  un2(d0, e0, e1); un2(d1, e2, e3);
-                  m0 = max3(m0, z[j], z[j + 1]); m1 = max3(m1, z[j + 2], z[j + 3]);
-                  e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
-                  d0 = pk2(e0, e1); d1 = pk2(e2, e3);
-                  s0 = add2(s0, d0); s1 = add2(s1, d1);
-                  if (CODE != PCPB_BF16) {
-                    const ulonglong2 y = v4[j / 4];
-                    un2(mul2(d0, y.x), e0, e1); un2(mul2(d1, y.y), e2, e3);
-                  }
-                  p[j / 2] = pack2(e0, e1); p[j / 2 + 1] = pack2(e2, e3);
-                }
-                top = fmaxf(m0, m1);
-                if (CODE == PCPB_BF16) top *= zscale;
-                sum = add2(s0, s1);
-                if (!__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) break;
-                raise(top, c);
-              }
-              l2 = add2(l2, sum);
-              tmem_st16(s_col(x) + lane_off + 16u * c, p);
-            };
+              for (int j = 0; j < 16; ++j) p[j] &= own == 2 * j ? 0xFFFF0000u : own == 2 * j + 1 ? 0x0000FFFFu : 0xFFFFFFFFu;
+            }
+            tmem_st16(s_col(x) + lane_off + 16u * c, p);
+          };
+          const int own = tree && A.a.null_self ? node - (tile - g.ct) * TILE : -1;       // a column that counts as a zero key and value
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
-              chunk(v, c);
-            }
-          } else {
-            uint32_t see[4] = {valid.x, valid.y, valid.z, valid.w};
-            if (tree) {
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(s_col(x) + lane_off + 32u * c, v);
+            const uint32_t word = tree ? anc[256 * ((tile - g.ct) * (TILE / 32) + c)] : c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
+            const int mine = own >= 32 * c && own < 32 * c + 32 ? own - 32 * c : -1;
+            if (!__all_sync(0xffffffffu, word == 0xffffffffu && mine < 0)) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) see[k] = anc[256 * ((tile - g.ct) * (TILE / 32) + k)];
+              for (int j = 0; j < 32; ++j) v[j] = j == mine ? 0u : (word >> j) & 1u ? v[j] : 0xFF800000u;
             }
-            const int own = tree && A.a.null_self ? node - (tile - g.ct) * TILE : -1;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t word = c == 0 ? see[0] : c == 1 ? see[1] : c == 2 ? see[2] : see[3];
-              uint32_t v[32], p[16];
-              tmem_ld32(s_col(x) + lane_off + 32u * c, v);
-              float top = -INFINITY;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float z = __uint_as_float(v[j]) * info[32 * c + j];
-                if (32 * c + j == own) z = 0.f;
-                z = (word >> j) & 1u ? z : -INFINITY;
-                top = fmaxf(top, z);
-                v[j] = __float_as_uint(z);
-              }
-              if (__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) raise(top, c);
-              const float ref = mref == -INFINITY ? 0.f : mref;
-              float add = 0.f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float e = ex2(__uint_as_float(v[j]) - ref);     // a masked column's weight is 0
-                add += e;
-                e = 32 * c + j != own && (word >> j) & 1u ? e * info[128 + 32 * c + j] : 0.f;
-                if (j & 1) p[j / 2] = pack2(__uint_as_float(p[j / 2]), e); else p[j / 2] = __float_as_uint(e);
-              }
-              l2 = add2(l2, pk2(add, 0.f));
-              tmem_st16(s_col(x) + lane_off + 16u * c, p);
-            }
+            chunk(v, c, mine);
           }
           tmem_st_wait();
         }
@@ -1126,22 +1130,30 @@ int check_heads(const pcpb_kv_cache& c, int n_head, int max_nodes, char* err, si
   return PCPB_OK;
 }
 
+template <int HD, int ROWS> cudaError_t launch_join(cudaStream_t st, const AttnArgs& A, int blocks) {
+  const int rows = A.a.max_nodes * A.G, items = A.c.n_kv_head * ((rows + ROWS - 1) / ROWS);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(A.c.batch, items, (min(rows, ROWS) + 15) / 16); cfg.blockDim = dim3(256); cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_tree_join<HD, ROWS>, A, blocks);
+}
 template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnArgs& A, int blocks) {
   const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)WARPS * RW * HD * 4;
   cudaError_t e = cudaFuncSetAttribute(k_tree_rows<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   k_tree_rows<HD, CODE><<<blocks, WARPS * 32, smem, st>>>(A);
-  const int items = A.c.n_kv_head * ((A.a.max_nodes * A.G + RW - 1) / RW);
-  k_tree_join<HD, RW><<<dim3(A.c.batch, items), 256, 0, st>>>(A, blocks);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  return e == cudaSuccess ? launch_join<HD, RW>(st, A, blocks) : e;
 }
 template <int HD, int CODE> cudaError_t launch_tc(cudaStream_t st, const AttnArgs& A, int blocks) {
   cudaError_t e = cudaFuncSetAttribute(k_tree_tc<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HD>::BYTES);
   if (e != cudaSuccess) return e;
   k_tree_tc<HD, CODE><<<blocks, TC_THREADS, TcCfg<HD>::BYTES, st>>>(A);
-  const int rows = A.a.max_nodes * A.G, items = A.c.n_kv_head * ((rows + TR - 1) / TR);
-  k_tree_join<HD, TR><<<dim3(A.c.batch, items, (min(rows, TR) + 15) / 16), 256, 0, st>>>(A, blocks);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  return e == cudaSuccess ? launch_join<HD, TR>(st, A, blocks) : e;
 }
 // Rows of a kv head from which on the tensor-core kernel takes over
 constexpr int TC_FROM = 17;

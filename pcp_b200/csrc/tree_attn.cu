@@ -35,6 +35,9 @@ struct AttnArgs {
   float* part_o;                     // [blocks][2][ROWS][HD]
 };
 
+// Programmatic dependent launch: the join's blocks may be set up while the attention kernel drains; they wait for its results themselves.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -116,17 +119,20 @@ __device__ __forceinline__ int seq_at(const long long* plan, int batch, long lon
   return lo;
 }
 
-// ---- the kernel for any number of rows: 16 a tile, mma.sync ---------------------------------------------------------
-// Eight warps share the 16 rows and split the keys in units of 16: no barrier until the item ends.  A lane's 16-byte pieces of keys
-// and values go straight from global memory into the fragments of mma.sync m16n8k16: which of the head_dim elements meet in one
-// k16 step does not matter as long as q is read with the same assignment, and which output columns a lane holds does not
-// matter as long as they are stored where they belong; so no element changes lanes.  Values are paired by position with byte
-// permutes.  The scores' fragment is the weights' operand of the second product as it stands.
-constexpr int RW = 16;               // rows of a tile
-constexpr int WARPS = 8;
+// ---- the kernel for few rows: 8 a tile, mma.sync ---------------------------------------------------------------------
+// The warps of a block share the 8 rows and split the keys in units of 16: no barrier until the item ends.  Keys and values are the 16-row
+// operands of mma.sync m16n8k16 (S^T = K Q^T, O^T = V^T P^T), the rows of q its 8 columns.  A lane's 16-byte pieces of keys and values are
+// what it needs as fragments: which of the head_dim elements meet in one k16 step does not matter as long as q is read with the
+// same assignment, and which output columns a lane holds does not matter as long as they are stored where they belong; so no element
+// changes lanes, and a lane reads back from shared memory only what it copied there itself.  Values are paired by position with
+// byte permutes, the weights change from accumulator to operand with movmatrix.
+// Bound: HBM, with the widening of 8-bit codes close behind.  Every warp keeps a ring of units in flight with cp.async (130 to 200 KB an
+// SM); the block-table entries are read one unit ahead of that.
+constexpr int RW = 8;                // rows of a tile
 
 template <int HD, int CODE> struct Frag {
   static constexpr int ES = CODE == PCPB_BF16 ? 2 : 1;
+  static constexpr int WARPS = CODE == PCPB_BF16 ? 8 : 16;
   static constexpr int KB = HD * ES / 4 < 16 ? HD * ES / 4 : 16, KE = KB / ES, KC = HD / (4 * KE);   // bytes, elements of a lane's key piece; pieces a row
   static constexpr int VB = HD * ES / 8 < 16 ? HD * ES / 8 : 16, VE = VB / ES, VC = HD / (8 * VE);
 };
@@ -135,107 +141,99 @@ template <int BYTES> __device__ __forceinline__ void ld_bytes(const void* p, uin
   else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
   else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {     // an 8 x 8 tile of 16-bit values, a row in four lanes
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
+// m, l: rows 2 qd, 2 qd + 1 (l: this lane's share); o[t][k]: row 2 qd + (k & 1), column out_col(t, g, k >> 1)
 template <int HD> struct RowState {
-  uint32_t q[HD / 16][4];
-  float o[HD / 8][4], m[2], l[2];
+  uint32_t q[HD / 16][2];
+  float o[HD / 16][4], m[2], l[2];
 };
+template <int HD, int CODE> __device__ __forceinline__ int out_col(int t, int g, int i) {
+  typedef Frag<HD, CODE> F;
+  return (t / (F::VE / 2)) * 8 * F::VE + g * F::VE + t % (F::VE / 2) * 2 + i;
+}
 
-// q fragments of rows row0 .. row0 + 15 in the element order of Frag<HD, CODE>
+// q fragments of rows row0 .. row0 + 7 (row g in the lanes 4 g ..) in the element order of Frag<HD, CODE>
 template <int HD, int CODE> __device__ __forceinline__ void load_q(const AttnArgs& A, const Seq& s, int kvh, int row0, RowState<HD>& R) {
   typedef Frag<HD, CODE> F;
-  const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3, rows = s.n * A.G;
+  const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3, r = row0 + g;
+  const bf16* p = (const bf16*)A.a.q + (long long)(s.n0 + r / A.G) * A.a.q_row + (long long)(kvh * A.G + r % A.G) * A.a.q_head;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = row0 + g + 8 * half;
-    const bf16* p = (const bf16*)A.a.q + (long long)(s.n0 + r / A.G) * A.a.q_row + (long long)(kvh * A.G + r % A.G) * A.a.q_head;
-#pragma unroll
-    for (int st = 0; st < HD / 16; ++st) {
-      const int e = 4 * F::KE * (st / (F::KE / 4)) + F::KE * qd + 4 * (st % (F::KE / 4));
-      const uint2 v = r < rows ? *reinterpret_cast<const uint2*>(p + e) : make_uint2(0u, 0u);
-      R.q[st][half] = v.x; R.q[st][2 + half] = v.y;
-    }
+  for (int st = 0; st < HD / 16; ++st) {
+    const int e = 4 * F::KE * (st / (F::KE / 4)) + F::KE * qd + 4 * (st % (F::KE / 4));
+    const uint2 v = r < s.n * A.G ? *reinterpret_cast<const uint2*>(p + e) : make_uint2(0u, 0u);
+    R.q[st][0] = v.x; R.q[st][1] = v.y;
   }
 }
 
-// Output columns of accumulator tile t: element k of the fragment is row g + 8 (k >> 1), column col(t, 2 qd + (k & 1))
-template <int HD, int CODE> __device__ __forceinline__ int out_col(int t, int n) {
-  typedef Frag<HD, CODE> F;
-  return (t / F::VE) * 8 * F::VE + n * F::VE + t % F::VE;
-}
-
-// One unit of 16 keys.  krow / vrow: this lane's rows of keys (positions g, g + 8 of the unit) and values (2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd),
-// NULL where there is none; keep[half][i]: may row g + 8 half attend the score fragment's column i (positions 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd);
-// zero[half][i]: that slot counts as a zero key and value.
+// One unit of 16 keys.  load_k(j, c, w), load_v(j, c, w): this lane's pieces of its rows of keys (positions g, g + 8 of the unit) and values
+// (2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd); zeros where there is no row.  ks, vs: scales of the positions g and g + 8.  keep: bit 2 i + j: may
+// row 2 qd + j attend position g + 8 i; zero: the same for slots that count as a zero key and value.
+// The reference maximum of a row moves only when a score passes it by 2^8, so that the outputs are rarely rescaled.
 // TREE: rows attend different keys of the unit.  A weight of 0 does not keep an infinity or a NaN of another branch's value out of the
-// matrix product, so a unit with such a value adds its products one by one, attended ones only.
-template <int HD, int CODE, bool TREE>
-__device__ __forceinline__ void unit(RowState<HD>& R, const uint8_t* const (&krow)[2], const uint8_t* const (&vrow)[4], const float (&ks)[4],
-                                     const float (&vs)[4], float zscale, const bool (&keep)[2][4], const bool (&zero)[2][4]) {
+// matrix product, so a unit with such a value adds its products one by one (vrow: the rows of the values), attended ones only.
+template <int HD, int CODE, bool TREE, typename LK, typename LV>
+__device__ __forceinline__ void unit(RowState<HD>& R, const LK& load_k, const LV& load_v, const uint8_t* const (&vrow)[4], const float (&ks)[2],
+                                     const float (&vs)[2], float zscale, uint32_t keep, uint32_t zero) {
   typedef Frag<HD, CODE> F;
   const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
-  uint32_t kw[2][F::KC][F::KB / 4], vw[4][F::VC][F::VB / 4];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};                            // s[2 i + j]: position g + 8 i, row 2 qd + j
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int c = 0; c < F::KC; ++c) {
+    uint32_t k0[F::KB / 4], k1[F::KB / 4];
+    load_k(0, c, k0);
+    load_k(1, c, k1);
 #pragma unroll
-    for (int c = 0; c < F::KC; ++c) {
-#pragma unroll
-      for (int i = 0; i < F::KB / 4; ++i) kw[j][c][i] = 0u;
-      if (krow[j]) ld_bytes<F::KB>(krow[j] + (4 * F::KE * c + F::KE * qd) * F::ES, kw[j][c]);
+    for (int sub = 0; sub < F::KE / 4; ++sub) {
+      const int st = c * (F::KE / 4) + sub;
+      uint32_t a[4];
+      if (CODE == PCPB_BF16) { a[0] = k0[(2 * sub) % (F::KB / 4)]; a[2] = k0[(2 * sub + 1) % (F::KB / 4)]; a[1] = k1[(2 * sub) % (F::KB / 4)]; a[3] = k1[(2 * sub + 1) % (F::KB / 4)]; }
+      else { widen4<CODE>(k0[sub % (F::KB / 4)], a[0], a[2]); widen4<CODE>(k1[sub % (F::KB / 4)], a[1], a[3]); }
+      mma16816(s, a, R.q[st][0], R.q[st][1]);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      s[2 * i + j] *= zscale * ks[i];
+      if (TREE && (zero >> (2 * i + j)) & 1u) s[2 * i + j] = 0.f;
+      if (!((keep >> (2 * i + j)) & 1u)) s[2 * i + j] = -INFINITY;
+    }
+  float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+  if (__any_sync(0xffffffffu, top[0] > R.m[0] + 8.f || top[1] > R.m[1] + 8.f || (R.m[0] == -INFINITY && top[0] > -INFINITY) || (R.m[1] == -INFINITY && top[1] > -INFINITY))) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+      const float m = R.m[j], to = fmaxf(m, top[j]), corr = m == -INFINITY ? 1.f : ex2(m - to);      // (nothing but zeros so far: any factor will do)
+      R.m[j] = to;
+      R.l[j] *= corr;
+#pragma unroll
+      for (int t = 0; t < HD / 16; ++t) { R.o[t][j] *= corr; R.o[t][2 + j] *= corr; }
+    }
+  }
+  float w[4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float ref = R.m[j] == -INFINITY ? 0.f : R.m[j];       // a row that has seen nothing yet: every weight is 0
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float e = ex2(s[2 * i + j] - ref);
+      R.l[j] += e;
+      w[2 * i + j] = TREE && (zero >> (2 * i + j)) & 1u ? 0.f : CODE == PCPB_BF16 ? e : e * vs[i];
+    }
+  }
+  const uint32_t b0 = transpose8(pack2(w[0], w[1])), b1 = transpose8(pack2(w[2], w[3]));
+  uint32_t vw[4][F::VC][F::VB / 4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int c = 0; c < F::VC; ++c) {
-#pragma unroll
-      for (int i = 0; i < F::VB / 4; ++i) vw[j][c][i] = 0u;
-      if (vrow[j]) ld_bytes<F::VB>(vrow[j] + (8 * F::VE * c + F::VE * g) * F::ES, vw[j][c]);
-    }
-  float s[2][4] = {};
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int st = 0; st < HD / 16; ++st) {
-      const int c = st / (F::KE / 4), sub = st % (F::KE / 4);
-      if (CODE == PCPB_BF16) {
-        mma16816(s[j], R.q[st], kw[j][c][(2 * sub) % (F::KB / 4)], kw[j][c][(2 * sub + 1) % (F::KB / 4)]);
-      } else {
-        uint32_t b0, b1;
-        widen4<CODE>(kw[j][c][sub % (F::KB / 4)], b0, b1);
-        mma16816(s[j], R.q[st], b0, b1);
-      }
-    }
-  // scores: s[j][2 half + i] is row g + 8 half, position 8 j + 2 qd + i
-  uint32_t p[4];
-  float corr[2], wt[2][4];
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float z[4], mx = R.m[half];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      z[i] = s[i >> 1][2 * half + (i & 1)] * (zscale * ks[i]);
-      if (zero[half][i]) z[i] = 0.f;
-      if (!keep[half][i]) z[i] = -INFINITY;
-      mx = fmaxf(mx, z[i]);
-    }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float ref = mx == -INFINITY ? 0.f : mx;               // a row that has seen nothing yet: every weight below is 0
-    corr[half] = ex2(R.m[half] - ref);
-    R.m[half] = mx;
-    float e[4], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e[i] = ex2(z[i] - ref);
-      sum += e[i];
-      e[i] = zero[half][i] ? 0.f : e[i] * vs[i];
-      if (TREE) wt[half][i] = bf16_round(e[i]);
-    }
-    R.l[half] = R.l[half] * corr[half] + sum;                   // this lane's share of the row's sum
-    p[half] = pack2(e[0], e[1]); p[2 + half] = pack2(e[2], e[3]);
-  }
-#pragma unroll
-  for (int t = 0; t < HD / 8; ++t) { R.o[t][0] *= corr[0]; R.o[t][1] *= corr[0]; R.o[t][2] *= corr[1]; R.o[t][3] *= corr[1]; }
+    for (int c = 0; c < F::VC; ++c) load_v(j, c, vw[j][c]);
   if (TREE) {
     bool odd = false;
 #pragma unroll
@@ -245,23 +243,22 @@ __device__ __forceinline__ void unit(RowState<HD>& R, const uint8_t* const (&kro
 #pragma unroll
         for (int i = 0; i < F::VB / 4; ++i) odd |= (vw[j][c][i] & 0x7F80u) == 0x7F80u || (vw[j][c][i] & 0x7F800000u) == 0x7F800000u;
     if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
 #pragma unroll 1
-        for (int x = 0; x < 4; ++x) {                           // key 8 (i >> 1) + 2 x + (i & 1): its weights are with lane x of the row's four
-          const int src = (lane & ~3) | x;
-          const bf16* v = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)vrow[i], src);
+      for (int pos = 0; pos < 16; ++pos) {                      // its weights are with the lanes 4 (pos & 7) + qd, its value's row with the lanes whose qd is x
+        const int src = (pos & 7) * 4 + qd, x = (pos & 7) >> 1;
+        const uint8_t* row = (pos & 8) ? ((pos & 1) ? vrow[3] : vrow[2]) : ((pos & 1) ? vrow[1] : vrow[0]);
+        const bf16* v = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)row, x);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float w = __shfl_sync(0xffffffffu, wt[half][i], src);
-            const int on = __shfl_sync(0xffffffffu, (int)(keep[half][i] && !zero[half][i]), src);
-            if (!on) continue;
+        for (int j = 0; j < 2; ++j) {
+          const float wt = __shfl_sync(0xffffffffu, bf16_round((pos & 8) ? w[2 + j] : w[j]), src);
+          const uint32_t on = __shfl_sync(0xffffffffu, keep & ~zero, src) >> (((pos & 8) ? 2 : 0) + j) & 1u;
+          if (!on) continue;
 #pragma unroll
-            for (int t = 0; t < HD / 8; ++t)
+          for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
-              for (int k = 0; k < 2; ++k) R.o[t][2 * half + k] += w * to_f(v[out_col<HD, CODE>(t, 2 * qd + k)]);
-          }
+            for (int i = 0; i < 2; ++i) R.o[t][2 * i + j] += wt * to_f(v[out_col<HD, CODE>(t, g, i)]);
         }
+      }
       return;
     }
   }
@@ -270,20 +267,21 @@ __device__ __forceinline__ void unit(RowState<HD>& R, const uint8_t* const (&kro
 #pragma unroll
     for (int i = 0; i < F::VB / 4; ++i) {
       if (CODE == PCPB_BF16) {
-        mma16816(R.o[c * F::VE + 2 * i], p, __byte_perm(vw[0][c][i], vw[1][c][i], 0x5410), __byte_perm(vw[2][c][i], vw[3][c][i], 0x5410));
-        mma16816(R.o[c * F::VE + 2 * i + 1], p, __byte_perm(vw[0][c][i], vw[1][c][i], 0x7632), __byte_perm(vw[2][c][i], vw[3][c][i], 0x7632));
+        const uint32_t a[4] = {__byte_perm(vw[0][c][i], vw[1][c][i], 0x5410), __byte_perm(vw[0][c][i], vw[1][c][i], 0x7632),
+                               __byte_perm(vw[2][c][i], vw[3][c][i], 0x5410), __byte_perm(vw[2][c][i], vw[3][c][i], 0x7632)};
+        mma16816(R.o[c * (F::VE / 2) + i], a, b0, b1);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t a0, a1, b0, b1;
-          widen4<CODE>(__byte_perm(vw[0][c][i], vw[1][c][i], h ? 0x7362 : 0x5140), a0, a1);
-          widen4<CODE>(__byte_perm(vw[2][c][i], vw[3][c][i], h ? 0x7362 : 0x5140), b0, b1);
-          mma16816(R.o[c * F::VE + 4 * i + 2 * h], p, a0, b0);
-          mma16816(R.o[c * F::VE + 4 * i + 2 * h + 1], p, a1, b1);
+          uint32_t a[4];
+          widen4<CODE>(__byte_perm(vw[0][c][i], vw[1][c][i], h ? 0x7362 : 0x5140), a[0], a[1]);
+          widen4<CODE>(__byte_perm(vw[2][c][i], vw[3][c][i], h ? 0x7362 : 0x5140), a[2], a[3]);
+          mma16816(R.o[c * (F::VE / 2) + 2 * i + h], a, b0, b1);
         }
       }
     }
 }
+
 // Ancestors-or-self of the nodes of a tile's rows, 256 bits a row, in shared memory
 __device__ void make_ancestors(const AttnArgs& A, const Seq& s, int row0, int rows_tile, int16_t* par, uint32_t (*anc)[MAX_NODES / 32]) {
   for (int i = threadIdx.x; i < s.n; i += blockDim.x) {
@@ -307,147 +305,182 @@ __device__ void make_ancestors(const AttnArgs& A, const Seq& s, int row0, int ro
   __syncthreads();
 }
 
-template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_tree_rows(const __grid_constant__ AttnArgs A) {
+template <int BYTES> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool on) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(on ? BYTES : 0), "n"(BYTES) : "memory");
+}
+// A warp's ring: stages of one unit (keys, values, 16 key scales, 16 value scales, the valid positions); the same memory holds the warp's part
+// of the outputs when the item ends.
+template <int HD, int CODE> struct Ring {
+  typedef Frag<HD, CODE> F;
+  static constexpr int K_BYTES = 16 * HD * F::ES, STAGE = 2 * K_BYTES + 144;
+  static constexpr int FIT = 204000 / F::WARPS / STAGE, NST = FIT < 6 ? FIT : 6;
+  static constexpr int OUT = RW * HD * 4, BYTES = NST * STAGE > OUT ? NST * STAGE : OUT;
+};
+
+template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WARPS * 32, 1) k_tree_rows(const __grid_constant__ AttnArgs A) {
+  typedef Frag<HD, CODE> F;
+  typedef Ring<HD, CODE> G;
+  constexpr int WARPS = F::WARPS;
   extern __shared__ __align__(16) uint8_t smem[];
   long long* plan = reinterpret_cast<long long*>(smem);                       // [batch + 1]
-  float* mo = reinterpret_cast<float*>(smem + ((A.c.batch + 1) * 8 + 15) / 16 * 16);   // [WARPS][RW][HD]
+  uint8_t* rings = smem + ((A.c.batch + 1) * 8 + 15) / 16 * 16;
   __shared__ float mml[WARPS][RW][2];
   __shared__ int16_t par[MAX_NODES];
   __shared__ uint32_t anc[RW][MAX_NODES / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;");
+  uint8_t* const ring = rings + warp * G::BYTES;
+  float* const mine = reinterpret_cast<float*>(ring);           // [RW][HD]
+  const uint32_t ring_s = smem_u32(ring);
+  pdl_launch_dependents();
   make_plan<RW>(A, plan);
   const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
   if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
   const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
   const float zscale = A.a.scale * LOG2E;
-  const bool none[2][4] = {};
   for (long long w = w0; w < w1;) {
     const int b = seq_at(plan, A.c.batch, w);
     const Seq s = seq_of(A, b);
     const int ct = tiles_of(s.ctx), T = ct + tiles_of(s.n), RT = (s.n * A.G + RW - 1) / RW;
-    const long long item = (w - plan[b]) / T;
-    const int t0 = (int)((w - plan[b]) % T), t1 = (int)min((long long)T, t0 + (w1 - w));
-    const int kvh = (int)(item / RT), row0 = (int)(item % RT) * RW, rows = s.n * A.G;
+    const long long at = w - plan[b], item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)T) : at / T;
+    const int t0 = (int)(at - item * T), t1 = (int)min((long long)T, t0 + (w1 - w));
+    const int kvh = (int)item / RT, row0 = ((int)item - kvh * RT) * RW, rows = s.n * A.G;
     RowState<HD> R;
 #pragma unroll
-    for (int t = 0; t < HD / 8; ++t) R.o[t][0] = R.o[t][1] = R.o[t][2] = R.o[t][3] = 0.f;
+    for (int t = 0; t < HD / 16; ++t) R.o[t][0] = R.o[t][1] = R.o[t][2] = R.o[t][3] = 0.f;
     R.m[0] = R.m[1] = -INFINITY; R.l[0] = R.l[1] = 0.f;
-    // cached keys [t0 TILE, t1 TILE)
-    if (t0 < ct) {
-      load_q<HD, CODE>(A, s, kvh, row0, R);
-      const int end = min(s.ctx, t1 * TILE);
-      constexpr int ES = Frag<HD, CODE>::ES;
-      for (int u = t0 * TILE + warp * 16; u < end; u += WARPS * 16) {
-        const int pos = u + (lane & 15);                        // lanes 0 .. 15 find the rows of the unit's positions
-        const int page = pos < end ? page_of(A.c, b, pos / A.c.page_tokens) : -1;
-        if (pos < end && page < 0) op_note(A.status, PCPB_OPS_BAD_PAGE);
-        const int in_page = pos % A.c.page_tokens;
-        const long long off = page < 0 ? -1 : page_row(page, A.c.page_stride, kvh, A.c.page_tokens, in_page, HD) * ES;
-        const long long soff = page < 0 ? -1 : page_row(page, A.c.scale_stride, kvh, A.c.page_tokens, in_page, 1);
-        const uint8_t *krow[2], *vrow[4];
-        float ks[4], vs[4];
-        bool keep[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const long long o = __shfl_sync(0xffffffffu, off, 8 * j + g);
-          krow[j] = o < 0 ? nullptr : (const uint8_t*)A.c.k + o;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = 8 * (i >> 1) + 2 * qd + (i & 1);
-          const long long o = __shfl_sync(0xffffffffu, off, at), so = __shfl_sync(0xffffffffu, soff, at);
-          vrow[i] = o < 0 ? nullptr : (const uint8_t*)A.c.v + o;
-          keep[0][i] = keep[1][i] = o >= 0;
-          ks[i] = vs[i] = 1.f;
-          if (CODE != PCPB_BF16 && o >= 0) { ks[i] = A.c.k_scale[so]; vs[i] = A.c.v_scale[so]; }
-        }
-        unit<HD, CODE, false>(R, krow, vrow, ks, vs, zscale, keep, none);
-      }
-    }
-    // the nodes' own keys
+    // the nodes' own keys (bf16)
     if (t1 > ct) {
       make_ancestors(A, s, row0, RW, par, anc);
       load_q<HD, PCPB_BF16>(A, s, kvh, row0, R);
-      RowState<HD> N;                                           // 8-bit caches: the nodes' keys are bf16, with their own order of q and columns
       const int lo = max(t0 - ct, 0) * TILE, end = min(s.n, (t1 - ct) * TILE);
-#pragma unroll
-      for (int t = 0; t < HD / 8; ++t) N.o[t][0] = N.o[t][1] = N.o[t][2] = N.o[t][3] = 0.f;
-#pragma unroll
-      for (int t = 0; t < HD / 16; ++t) for (int i = 0; i < 4; ++i) N.q[t][i] = R.q[t][i];
-      N.m[0] = N.m[1] = -INFINITY; N.l[0] = N.l[1] = 0.f;
-      const float one[4] = {1.f, 1.f, 1.f, 1.f};
+      const float one[2] = {1.f, 1.f};
+      typedef Frag<HD, PCPB_BF16> B;
       for (int u = lo + warp * 16; u < end; u += WARPS * 16) {
         const uint8_t *krow[2], *vrow[4];
-        bool keep[2][4], zero[2][4];
+        uint32_t keep = 0, zero = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int i = u + 8 * j + g;
-          krow[j] = i < end ? (const uint8_t*)((const bf16*)A.a.k + (long long)(s.n0 + i) * A.a.k_row + (long long)kvh * A.a.k_head) : nullptr;
+        for (int i = 0; i < 2; ++i) {
+          const int at = u + 8 * i + g;
+          krow[i] = at < end ? (const uint8_t*)((const bf16*)A.a.k + (long long)(s.n0 + at) * A.a.k_row + (long long)kvh * A.a.k_head) : nullptr;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = 2 * qd + j;
+            if (at < end && ((anc[r][(at >> 5) & 7] >> (at & 31)) & 1u)) keep |= 1u << (2 * i + j);
+            if (A.a.null_self && at == (row0 + r) / A.G) zero |= 1u << (2 * i + j);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = u + 8 * (j >> 1) + 2 * qd + (j & 1);
           vrow[j] = i < end ? (const uint8_t*)((const bf16*)A.a.v + (long long)(s.n0 + i) * A.a.v_row + (long long)kvh * A.a.v_head) : nullptr;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = g + 8 * half;
-            keep[half][j] = i < end && ((anc[r][(i >> 5) & 7] >> (i & 31)) & 1u);
-            zero[half][j] = A.a.null_self && i == (row0 + r) / A.G;
-          }
         }
-        unit<HD, PCPB_BF16, true>(N, krow, vrow, one, one, zscale, keep, zero);
+        auto zeros = [](uint32_t* w, int n) { for (int i = 0; i < n; ++i) w[i] = 0u; };
+        auto load_k = [&](int j, int c, uint32_t (&w)[B::KB / 4]) { zeros(w, B::KB / 4); if (krow[j]) ld_bytes<B::KB>(krow[j] + (4 * B::KE * c + B::KE * qd) * 2, w); };
+        auto load_v = [&](int j, int c, uint32_t (&w)[B::VB / 4]) { zeros(w, B::VB / 4); if (vrow[j]) ld_bytes<B::VB>(vrow[j] + (8 * B::VE * c + B::VE * g) * 2, w); };
+        unit<HD, PCPB_BF16, true>(R, load_k, load_v, vrow, one, one, zscale, keep, zero);
       }
-      // join both parts: through shared memory, since the columns of a lane differ between the two
-      if (CODE != PCPB_BF16) {
+      if (CODE != PCPB_BF16) {                                  // from a lane's columns of the bf16 form to those of the codes' form
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float m = fmaxf(R.m[half], N.m[half]), ref = m == -INFINITY ? 0.f : m;
-          const float cr = ex2(R.m[half] - ref), cn = ex2(N.m[half] - ref);
-          R.l[half] = R.l[half] * cr + N.l[half] * cn; R.m[half] = m;
-          float* row = mo + ((size_t)warp * RW + g + 8 * half) * HD;
+        for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
-          for (int t = 0; t < HD / 8; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              row[out_col<HD, PCPB_BF16>(t, 2 * qd + i)] = N.o[t][2 * half + i] * cn;
-              R.o[t][2 * half + i] *= cr;
-            }
-        }
+          for (int k = 0; k < 4; ++k) mine[(2 * qd + (k & 1)) * HD + out_col<HD, PCPB_BF16>(t, g, k >> 1)] = R.o[t][k];
         __syncwarp();
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
-          for (int t = 0; t < HD / 8; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              R.o[t][2 * half + i] += mo[((size_t)warp * RW + g + 8 * half) * HD + out_col<HD, CODE>(t, 2 * qd + i)];
+          for (int k = 0; k < 4; ++k) R.o[t][k] = mine[(2 * qd + (k & 1)) * HD + out_col<HD, CODE>(t, g, k >> 1)];
         __syncwarp();
-      } else {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float m = fmaxf(R.m[half], N.m[half]), ref = m == -INFINITY ? 0.f : m;
-          const float cr = ex2(R.m[half] - ref), cn = ex2(N.m[half] - ref);
-          R.l[half] = R.l[half] * cr + N.l[half] * cn; R.m[half] = m;
-#pragma unroll
-          for (int t = 0; t < HD / 8; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) R.o[t][2 * half + i] = R.o[t][2 * half + i] * cr + N.o[t][2 * half + i] * cn;
-        }
       }
     }
-    // the eight warps' parts -> the tile's rows
+    // cached keys [t0 TILE, t1 TILE)
+    if (t0 < ct) {
+      const int end = min(s.ctx, t1 * TILE), first = t0 * TILE + warp * 16;
+      const int nu = first < end ? (end - first + WARPS * 16 - 1) / (WARPS * 16) : 0;      // this warp's units
+      struct Entry { int raw, in; };
+      auto look = [&](int k) {                                  // lanes l and l + 16 look up position l of unit k
+        Entry e{-1, -1};
+        const int pos = first + k * (WARPS * 16) + (lane & 15);
+        if (k < nu && pos < end) {
+          const int lp = pos / A.c.page_tokens;
+          e.in = pos - lp * A.c.page_tokens;
+          e.raw = __ldg(A.c.block_table + (size_t)b * A.c.max_pages + lp);           // lp < max_pages: ctx is clipped to the table
+        }
+        return e;
+      };
+      auto issue = [&](int k, const Entry& e) {
+        const int page = clip_page(e.raw, A.c.n_pages);
+        if (e.in >= 0 && page < 0) op_note(A.status, PCPB_OPS_BAD_PAGE);
+        const long long off = page < 0 ? -1 : page_row(page, A.c.page_stride, kvh, A.c.page_tokens, e.in, HD) * F::ES;
+        const uint32_t st = ring_s + (k % G::NST) * G::STAGE;
+        const uint32_t valid = __ballot_sync(0xffffffffu, off >= 0) & 0xFFFFu;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float l = R.l[half];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (qd == 0) { mml[warp][g + 8 * half][0] = R.m[half]; mml[warp][g + 8 * half][1] = l; }
+        for (int j = 0; j < 2; ++j) {
+          const long long o = __shfl_sync(0xffffffffu, off, 8 * j + g);
 #pragma unroll
-      for (int t = 0; t < HD / 8; ++t)
+          for (int c = 0; c < F::KC; ++c)
+            cp_async<F::KB>(st + ((j * F::KC + c) * 32 + lane) * F::KB, (const uint8_t*)A.c.k + (o < 0 ? 0 : o + (4 * F::KE * c + F::KE * qd) * F::ES), o >= 0);
+        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) mo[((size_t)warp * RW + g + 8 * half) * HD + out_col<HD, CODE>(t, 2 * qd + i)] = R.o[t][2 * half + i];
+        for (int j = 0; j < 4; ++j) {
+          const long long o = __shfl_sync(0xffffffffu, off, 8 * (j >> 1) + 2 * qd + (j & 1));
+#pragma unroll
+          for (int c = 0; c < F::VC; ++c)
+            cp_async<F::VB>(st + G::K_BYTES + ((j * F::VC + c) * 32 + lane) * F::VB, (const uint8_t*)A.c.v + (o < 0 ? 0 : o + (8 * F::VE * c + F::VE * g) * F::ES), o >= 0);
+        }
+        if (CODE != PCPB_BF16)
+          cp_async<4>(st + 2 * G::K_BYTES + lane * 4,
+                      (lane < 16 ? A.c.k_scale : A.c.v_scale) + (page < 0 ? 0 : page_row(page, A.c.scale_stride, kvh, A.c.page_tokens, e.in, 1)), page >= 0);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (k % G::NST) * G::STAGE + 2 * G::K_BYTES + 128) = valid;
+      };
+      Entry pre[G::NST];
+#pragma unroll
+      for (int k = 0; k < G::NST; ++k) pre[k] = look(k);
+#pragma unroll
+      for (int k = 0; k < G::NST - 1; ++k) {
+        if (k < nu) issue(k, pre[k]);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      Entry next = pre[G::NST - 1];
+      load_q<HD, CODE>(A, s, kvh, row0, R);
+#pragma unroll 1
+      for (int k = 0; k < nu; ++k) {
+        if (k + G::NST - 1 < nu) issue(k + G::NST - 1, next);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next = look(k + G::NST);
+        asm volatile("cp.async.wait_group %0;" ::"n"(G::NST - 1) : "memory");
+        __syncwarp();
+        const uint8_t* st = ring + (k % G::NST) * G::STAGE;
+        const float* sc = reinterpret_cast<const float*>(st + 2 * G::K_BYTES);
+        const uint32_t valid = *reinterpret_cast<const uint32_t*>(sc + 32);
+        float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+        uint32_t keep = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          keep |= ((valid >> (g + 8 * i)) & 1u) * (3u << (2 * i));
+          if (CODE != PCPB_BF16) { ks[i] = sc[g + 8 * i]; vs[i] = sc[16 + g + 8 * i]; }
+        }
+        auto load_k = [&](int j, int c, uint32_t (&w)[F::KB / 4]) { ld_bytes<F::KB>(st + ((j * F::KC + c) * 32 + lane) * F::KB, w); };
+        auto load_v = [&](int j, int c, uint32_t (&w)[F::VB / 4]) { ld_bytes<F::VB>(st + G::K_BYTES + ((j * F::VC + c) * 32 + lane) * F::VB, w); };
+        const uint8_t* const no_rows[4] = {};
+        unit<HD, CODE, false>(R, load_k, load_v, no_rows, ks, vs, zscale, keep, 0u);
+        __syncwarp();                                           // scales and valid positions are read by other lanes than wrote them
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
     }
+    // the warps' parts -> the tile's rows
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float l = R.l[j];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (g == 0) { mml[warp][2 * qd + j][0] = R.m[j]; mml[warp][2 * qd + j][1] = l; }
+    }
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mine[(2 * qd + (k & 1)) * HD + out_col<HD, CODE>(t, g, k >> 1)] = R.o[t][k];
     __syncthreads();
     const bool whole = t0 == 0 && t1 == T;
     const size_t slot = (size_t)blockIdx.x * 2 + (w == w0 ? 0 : 1);
@@ -462,7 +495,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_t
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) {
         const float f = ex2(mml[k][r][0] - ref);
-        const float4 v = *reinterpret_cast<const float4*>(mo + ((size_t)k * RW + r) * HD + c);
+        const float4 v = *reinterpret_cast<const float4*>(rings + k * G::BYTES + (r * HD + c) * 4);
         l += f * mml[k][r][1];
         o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
       }
@@ -482,10 +515,6 @@ template <int HD, int CODE> __global__ void __launch_bounds__(WARPS * 32, 1) k_t
   }
 }
 
-// Programmatic dependent launch: the join's blocks may be set up while the attention kernel drains; they wait for its results themselves.
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Adds up the parts of the items that were split.  grid = (batch, n_kv_head * most row tiles, ROWS / 16): a block joins 16 rows, a thread
 // four columns of one or more of them.
 template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ AttnArgs A, int blocks) {
@@ -501,7 +530,7 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
   if (P.c0 == P.c1) return;
   for (int i = threadIdx.x; i < 16 * (HD / 4); i += blockDim.x) {
     const int r = r0 + i / (HD / 4), c = i % (HD / 4) * 4;
-    if (row0 + r >= rows) continue;
+    if (r >= ROWS || row0 + r >= rows) continue;
     float m = -INFINITY, l = 0.f, o[4] = {};
     for (int k0 = P.c0; k0 <= P.c1; k0 += 4) {                  // four parts in flight, taken in block order
       float2 q[4];
@@ -1141,10 +1170,10 @@ template <int HD, int ROWS> cudaError_t launch_join(cudaStream_t st, const AttnA
   return cudaLaunchKernelEx(&cfg, k_tree_join<HD, ROWS>, A, blocks);
 }
 template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnArgs& A, int blocks) {
-  const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)WARPS * RW * HD * 4;
+  const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(k_tree_rows<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  k_tree_rows<HD, CODE><<<blocks, WARPS * 32, smem, st>>>(A);
+  k_tree_rows<HD, CODE><<<blocks, Frag<HD, CODE>::WARPS * 32, smem, st>>>(A);
   e = cudaGetLastError();
   return e == cudaSuccess ? launch_join<HD, RW>(st, A, blocks) : e;
 }
@@ -1156,7 +1185,7 @@ template <int HD, int CODE> cudaError_t launch_tc(cudaStream_t st, const AttnArg
   return e == cudaSuccess ? launch_join<HD, TR>(st, A, blocks) : e;
 }
 // Rows of a kv head from which on the tensor-core kernel takes over
-constexpr int TC_FROM = 17;
+constexpr int TC_FROM = 9;
 bool use_tc(const pcpb_kv_cache& c, int G, int max_nodes) { return c.head_dim != 32 && max_nodes * G >= TC_FROM; }
 template <int HD, int CODE> cudaError_t launch_any(cudaStream_t st, const AttnArgs& A, int blocks) {
   if constexpr (HD != 32)

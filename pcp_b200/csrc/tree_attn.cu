@@ -14,6 +14,8 @@
 // one it ends in) and k_tree_join adds them up in block order, so results do not depend on timing.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "decode_ops.h"
 #include "tc_common.cuh"
@@ -61,21 +63,53 @@ __device__ __forceinline__ uint32_t bsub2(uint32_t a, uint32_t b) {
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+__device__ __forceinline__ void mma16816_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // Four codes in a word -> two pairs of bf16 (exact: both code types have fewer significant bits than bf16).
 //   e4m3: sign and the seven other bits move to the bf16 fields of the same name; the exponent's bias then differs by
 //         127 - 7 = 120, which one product with 2^120 repairs, for subnormal codes as well.
 //   i8:   with c7 the sign bit and c the other seven, 0x4300 + c is 128 + c and 0x4300 + (c7 << 7) is 128 or 256; the code is their difference.
 template <int CODE> __device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
   if (CODE == PCPB_E4M3) {
-    const uint32_t t0 = __byte_perm(w, 0, 0x1404), t1 = __byte_perm(w, 0, 0x3424);
-    p01 = bmul2(((t0 >> 4) & 0x07F007F0u) | (t0 & 0x80008000u), 0x7B807B80u);
-    p23 = bmul2(((t1 >> 4) & 0x07F007F0u) | (t1 & 0x80008000u), 0x7B807B80u);
+    const uint32_t hi = (w & 0x80808080u) | ((w >> 4) & 0x07070707u), lo = (w << 4) & 0xF0F0F0F0u;    // the high and the low bytes of the four
+    p01 = bmul2(__byte_perm(lo, hi, 0x5140), 0x7B807B80u);
+    p23 = bmul2(__byte_perm(lo, hi, 0x7362), 0x7B807B80u);
   } else {
     const uint32_t t0 = __byte_perm(w, 0, 0x4140), t1 = __byte_perm(w, 0, 0x4342);
     p01 = bsub2((t0 & 0x007F007Fu) | 0x43004300u, (t0 & 0x00800080u) | 0x43004300u);
     p23 = bsub2((t1 & 0x007F007Fu) | 0x43004300u, (t1 & 0x00800080u) | 0x43004300u);
   }
 }
+
+// Four codes in a word -> two pairs of f16 (exact as well), which takes fewer operations: e4m3 has an instruction, and with u = code + 128 in
+// the low byte of 1024's bit pattern an i8 code is (1024 + u) - 1152.  Keys are widened this way, against q in f16; values are not, because
+// the weights they meet (times the values' scales) need bf16's range.
+template <int CODE> __device__ __forceinline__ void widen4_f16(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  if (CODE == PCPB_E4M3) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(p01), "=r"(p23) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p01) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p23) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
+  }
+}
+// Rows of bf16 become f16 times a power of two that puts the row's largest magnitude into [2^15, 2^16): exact for elements down to 2^-29 of it,
+// and off by at most 2^-40 of it below.  exp15: 15 - exponent of the largest magnitude (bit pattern `top` of its bf16); rows with an
+// infinity or a NaN are not scaled (their scores are not numbers either way).
+__device__ __forceinline__ int exp15(uint32_t top) {
+  const int e = (int)(top >> 7) - 127;
+  return e > 127 ? 0 : 15 - max(e, -100);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }       // -126 <= e <= 127
+__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w, float f) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(bf_hi(w) * f), "f"(bf_lo(w) * f));
+  return d;
+}
+__device__ __forceinline__ uint32_t top_abs2(uint32_t m, uint32_t w) { return max(m, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu)); }
 
 // Clipped lengths of sequence b.
 typedef SeqLen Seq;
@@ -147,10 +181,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {     // an 8 x 8 til
   return y;
 }
 
-// m, l: rows 2 qd, 2 qd + 1 (l: this lane's share); o[t][k]: row 2 qd + (k & 1), column out_col(t, g, k >> 1)
+// m, l, zs: rows 2 qd, 2 qd + 1 (l: this lane's share); o[t][k]: row 2 qd + (k & 1), column out_col(t, g, k >> 1)
 template <int HD> struct RowState {
   uint32_t q[HD / 16][2];
-  float o[HD / 16][4], m[2], l[2];
+  float o[HD / 16][4], m[2], l[2], zs[2];                        // zs: factor of a row's scores
 };
 template <int HD, int CODE> __device__ __forceinline__ int out_col(int t, int g, int i) {
   typedef Frag<HD, CODE> F;
@@ -168,6 +202,19 @@ template <int HD, int CODE> __device__ __forceinline__ void load_q(const AttnArg
     const uint2 v = r < s.n * A.G ? *reinterpret_cast<const uint2*>(p + e) : make_uint2(0u, 0u);
     R.q[st][0] = v.x; R.q[st][1] = v.y;
   }
+  R.zs[0] = R.zs[1] = A.a.scale * LOG2E;
+  if (CODE != PCPB_BF16) {                                      // q in f16, scaled by a power of two per row
+    uint32_t top = 0;
+#pragma unroll
+    for (int st = 0; st < HD / 16; ++st) top = top_abs2(top_abs2(top, R.q[st][0]), R.q[st][1]);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = exp15(top);
+#pragma unroll
+    for (int st = 0; st < HD / 16; ++st) { R.q[st][0] = bf16x2_to_f16x2(R.q[st][0], pow2(e)); R.q[st][1] = bf16x2_to_f16x2(R.q[st][1], pow2(e)); }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) R.zs[j] *= pow2(-__shfl_sync(0xffffffffu, e, 4 * (2 * qd + j)));
+  }
 }
 
 // One unit of 16 keys.  load_k(j, c, w), load_v(j, c, w): this lane's pieces of its rows of keys (positions g, g + 8 of the unit) and values
@@ -178,7 +225,7 @@ template <int HD, int CODE> __device__ __forceinline__ void load_q(const AttnArg
 // matrix product, so a unit with such a value adds its products one by one (vrow: the rows of the values), attended ones only.
 template <int HD, int CODE, bool TREE, typename LK, typename LV>
 __device__ __forceinline__ void unit(RowState<HD>& R, const LK& load_k, const LV& load_v, const uint8_t* const (&vrow)[4], const float (&ks)[2],
-                                     const float (&vs)[2], float zscale, uint32_t keep, uint32_t zero) {
+                                     const float (&vs)[2], uint32_t keep, uint32_t zero) {
   typedef Frag<HD, CODE> F;
   const int lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
   float s[4] = {0.f, 0.f, 0.f, 0.f};                            // s[2 i + j]: position g + 8 i, row 2 qd + j
@@ -192,15 +239,16 @@ __device__ __forceinline__ void unit(RowState<HD>& R, const LK& load_k, const LV
       const int st = c * (F::KE / 4) + sub;
       uint32_t a[4];
       if (CODE == PCPB_BF16) { a[0] = k0[(2 * sub) % (F::KB / 4)]; a[2] = k0[(2 * sub + 1) % (F::KB / 4)]; a[1] = k1[(2 * sub) % (F::KB / 4)]; a[3] = k1[(2 * sub + 1) % (F::KB / 4)]; }
-      else { widen4<CODE>(k0[sub % (F::KB / 4)], a[0], a[2]); widen4<CODE>(k1[sub % (F::KB / 4)], a[1], a[3]); }
-      mma16816(s, a, R.q[st][0], R.q[st][1]);
+      else { widen4_f16<CODE>(k0[sub % (F::KB / 4)], a[0], a[2]); widen4_f16<CODE>(k1[sub % (F::KB / 4)], a[1], a[3]); }
+      if (CODE == PCPB_BF16) mma16816(s, a, R.q[st][0], R.q[st][1]);
+      else mma16816_f16(s, a, R.q[st][0], R.q[st][1]);
     }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      s[2 * i + j] *= zscale * ks[i];
+      s[2 * i + j] *= R.zs[j] * ks[i];
       if (TREE && (zero >> (2 * i + j)) & 1u) s[2 * i + j] = 0.f;
       if (!((keep >> (2 * i + j)) & 1u)) s[2 * i + j] = -INFINITY;
     }
@@ -337,7 +385,6 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
   const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
   if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
   const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
-  const float zscale = A.a.scale * LOG2E;
   for (long long w = w0; w < w1;) {
     const int b = seq_at(plan, A.c.batch, w);
     const Seq s = seq_of(A, b);
@@ -378,7 +425,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
         auto zeros = [](uint32_t* w, int n) { for (int i = 0; i < n; ++i) w[i] = 0u; };
         auto load_k = [&](int j, int c, uint32_t (&w)[B::KB / 4]) { zeros(w, B::KB / 4); if (krow[j]) ld_bytes<B::KB>(krow[j] + (4 * B::KE * c + B::KE * qd) * 2, w); };
         auto load_v = [&](int j, int c, uint32_t (&w)[B::VB / 4]) { zeros(w, B::VB / 4); if (vrow[j]) ld_bytes<B::VB>(vrow[j] + (8 * B::VE * c + B::VE * g) * 2, w); };
-        unit<HD, PCPB_BF16, true>(R, load_k, load_v, vrow, one, one, zscale, keep, zero);
+        unit<HD, PCPB_BF16, true>(R, load_k, load_v, vrow, one, one, keep, zero);
       }
       if (CODE != PCPB_BF16) {                                  // from a lane's columns of the bf16 form to those of the codes' form
 #pragma unroll
@@ -463,7 +510,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
         auto load_k = [&](int j, int c, uint32_t (&w)[F::KB / 4]) { ld_bytes<F::KB>(st + ((j * F::KC + c) * 32 + lane) * F::KB, w); };
         auto load_v = [&](int j, int c, uint32_t (&w)[F::VB / 4]) { ld_bytes<F::VB>(st + G::K_BYTES + ((j * F::VC + c) * 32 + lane) * F::VB, w); };
         const uint8_t* const no_rows[4] = {};
-        unit<HD, CODE, false>(R, load_k, load_v, no_rows, ks, vs, zscale, keep, 0u);
+        unit<HD, CODE, false>(R, load_k, load_v, no_rows, ks, vs, keep, 0u);
         __syncwarp();                                           // scales and valid positions are read by other lanes than wrote them
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -569,9 +616,9 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
 // the products of one run while the other's softmax does: with more than 128 rows the streams are the two row tiles, which share
 // every tile of keys; with fewer both streams have the same rows and take the tiles of keys in turn, and are joined at the end.
 //   loaders (4 warps for keys, 4 for values)   find the rows of a tile's 128 positions in the block table, two tiles ahead, and bring them into
-//                       128-byte-swizzled shared memory as bf16.  8-bit codes are widened on the way: a thread holds its pieces of
-//                       the next tile in registers and loads a piece of the tile after as soon as it has widened one.  The key
-//                       loaders also describe the tile (scales, valid positions) in a ring.
+//                       128-byte-swizzled shared memory.  8-bit codes are widened on the way (keys to f16, values to bf16); a thread
+//                       holds its pieces of the next tile in registers meanwhile.  The key loaders also describe the tile (scales,
+//                       valid positions) in a ring.
 //   softmax (2 x 4)     a thread owns a row: scores from tensor memory, running maximum and sum, weights as bf16 over the scores.  The first
 //                       warp of each stream also issues its products when the four warps' weights are there: O += P V (P in tensor
 //                       memory, V as the MN-major operand), then S = Q K^T of the stream's next tile; it would only wait for them
@@ -594,7 +641,8 @@ template <int HD> struct TcCfg {
   static constexpr int OFF_ML = OFF_ROW + 4 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
   static constexpr int OFF_PAR = OFF_ML + 2 * 128 * 2 * 4;                // parents
   static constexpr int OFF_ANC = OFF_PAR + MAX_NODES * 2;                 // [MAX_NODES / 32][256] ancestors-or-self of the rows' nodes
-  static constexpr int OFF_BAR = OFF_ANC + MAX_NODES / 32 * 256 * 4;
+  static constexpr int OFF_QF = OFF_ANC + MAX_NODES / 32 * 256 * 4;       // [256] factors of the rows of q
+  static constexpr int OFF_BAR = OFF_QF + 256 * 4;
   static constexpr int OFF_PLAN = OFF_BAR + 256;
   static constexpr int BYTES = OFF_PLAN + (MAX_BATCH + 1) * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory");
@@ -758,15 +806,18 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       for (int i = 0; i < nt; ++i, ++gi) {
         const int tile = g.t0 + i, st = gi & 1, in = gi % INFO;
         const bool cached = tile < g.ct;
+        float* info = nullptr;
         if (!vals) {                                            // description of the tile
           wait_empty(iempty(in), ((gi / INFO) & 1) ^ 1);
-          float* info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
-          const float factor = f0.ks * (fabsf(A.a.scale) * LOG2E);
-          info[t] = factor < 1.17549435e-38f ? 1.17549435e-38f : factor;           // (a NaN stays)
+          info = reinterpret_cast<float*>(gen + Cfg::OFF_INFO + in * Cfg::INFO_BYTES);
           info[128 + t] = f0.vs;
           const uint32_t valid = __ballot_sync(0xffffffffu, f0.off >= 0);
           if (lane == 0) reinterpret_cast<uint32_t*>(info)[256 + (t >> 5)] = valid;
-          mbar_arrive(ifull(in));
+          if (cached || CODE == PCPB_BF16) {                    // (the nodes' key factors are known when their rows are there)
+            const float factor = f0.ks * (fabsf(A.a.scale) * LOG2E);
+            info[t] = factor < 1.17549435e-38f ? 1.17549435e-38f : factor;           // (a NaN stays)
+            mbar_arrive(ifull(in));
+          }
         }
         // the next tile's rows, and the pages of the one after
         if (i + 1 < nt) { rowoff[(st ^ 1) * 128 + t] = f1.off; }
@@ -789,20 +840,29 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           pending = full;
         } else if (cached) {
           const bool more = i + 1 < nt && tile + 1 < g.ct;
+          auto fill = [&](auto is_values) {
 #pragma unroll
           for (int k = 0; k < NP; ++k) {
             const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
             uint32_t p[8];
             constexpr int CC = CODE == PCPB_BF16 ? PCPB_I8 : CODE;
             const uint4 r = cur[CODE == PCPB_BF16 ? 0 : k];
-            widen4<CC>(r.x, p[0], p[1]); widen4<CC>(r.y, p[2], p[3]); widen4<CC>(r.z, p[4], p[5]); widen4<CC>(r.w, p[6], p[7]);
-            if (more) cur[CODE == PCPB_BF16 ? 0 : k] = piece(k, st ^ 1);
+            if constexpr (decltype(is_values)::value) { widen4<CC>(r.x, p[0], p[1]); widen4<CC>(r.y, p[2], p[3]); widen4<CC>(r.z, p[4], p[5]); widen4<CC>(r.w, p[6], p[7]); }
+            else { widen4_f16<CC>(r.x, p[0], p[1]); widen4_f16<CC>(r.y, p[2], p[3]); widen4_f16<CC>(r.z, p[4], p[5]); widen4_f16<CC>(r.w, p[6], p[7]); }
             const int flip = (c >> 2) & 1;                      // pieces of the second half go the other way round: other banks than the first half's
             st_shared16(dst + sw_off(row, 2 * c + flip), p[flip ? 4 : 0], p[flip ? 5 : 1], p[flip ? 6 : 2], p[flip ? 7 : 3]);
             st_shared16(dst + sw_off(row, 2 * c + 1 - flip), p[flip ? 0 : 4], p[flip ? 1 : 5], p[flip ? 2 : 6], p[flip ? 3 : 7]);
           }
+          };
+          if (vals) fill(std::true_type()); else fill(std::false_type());
           fence_proxy_async_smem();
           mbar_arrive(full);
+          // All of the next tile's loads together, after the last use of this one's: loads that are issued between uses of earlier ones share
+          // their scoreboards, and every use then waits for the newest load (1000 cycles a piece).
+          if (more) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) cur[CODE == PCPB_BF16 ? 0 : k] = piece(k, st ^ 1);
+          }
         } else {
           // rows of the nodes (bf16); values that are not numbers are left out and their nodes marked
           const int n0 = (tile - g.ct) * TILE;
@@ -832,10 +892,21 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
                   if ((q[j] & 0x7F800000u) == 0x7F800000u) { q[j] &= 0x0000FFFFu; bad = true; }
                 }
                 if (bad) atomicOr(&odd[seg & 3][(node >> 5) & 7], 1u << (node & 31));
+              } else if (CODE != PCPB_BF16) {                   // keys in f16, scaled by a power of two per row; PB lanes hold a row
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = top_abs2(top, q[j]);
+#pragma unroll
+                for (int o = PB / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int e = exp15(top);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[j] = bf16x2_to_f16x2(q[j], pow2(e));
+                if (idx % PB == 0) info[row] = fmaxf(pow2(-e) * (fabsf(A.a.scale) * LOG2E), 1.17549435e-38f);
               }
               st_shared16(dst + sw_off(row, idx % PB), q[0], q[1], q[2], q[3]);
             }
           }
+          if (!vals && CODE != PCPB_BF16) mbar_arrive(ifull(in));
           fence_proxy_async_smem();
           mbar_arrive(full);
         }
@@ -851,12 +922,14 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     // a negative scale changes the sign of q instead; a positive factor at least, so that a masked score stays -inf
     const float zscale = fmaxf(fabsf(A.a.scale) * LOG2E, 1.17549435e-38f);
     const uint32_t qsign = A.a.scale < 0.f ? 0x80008000u : 0u;
-    constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t KT = CODE == PCPB_BF16 ? 1u : 0u;        // type of both operands of the scores: bf16, or f16 for codes
+    constexpr uint32_t ID_S = (1u << 4) | (KT << 7) | (KT << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     const bool issuer = q4 == 0;
     int gi = 0, seg = 0, sn = 0;                                // tiles, segments; score tiles of this stream so far
     int16_t* par = reinterpret_cast<int16_t*>(gen + Cfg::OFF_PAR);
     float* ml = reinterpret_cast<float*>(gen + Cfg::OFF_ML);
+    float* qfac = reinterpret_cast<float*>(gen + Cfg::OFF_QF);
     uint32_t* anc = reinterpret_cast<uint32_t*>(gen + Cfg::OFF_ANC) + threadIdx.x;       // this thread's row: word k at anc[256 k]
     for (long long w = w0; w < w1; ++seg) {
       const Seg g = seg_at(A, plan, w, w1);
@@ -872,16 +945,32 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         if (bad) op_note(A.status, PCPB_OPS_BAD_TREE);
       }
       {
-        const bf16* src = (const bf16*)A.a.q + (long long)(g.s.n0 + node) * A.a.q_row + (long long)head * A.a.q_head;
-        const uint32_t dst = sQ + (pair ? x * Cfg::TILE_BYTES : 0);
-        const int c0 = pair ? 0 : x * (HD / 16), c1 = pair ? HD / 8 : c0 + HD / 16;
+        // rows of q: HD / 8 lanes a row, eight rows of a thread in flight; rows of both tiles, or all 256 threads on the one tile
+        constexpr int PQ = HD / 8, RP = 256 / PQ;               // rows of a pass
+        const int c = threadIdx.x % PQ, passes = (pair ? 256 : 128) / RP;
 #pragma unroll 1
-        for (int c = c0; c < c1; c += HD / 16) {                // HD / 16 pieces in flight
-          uint4 v[HD / 16];
+        for (int p0 = 0; p0 < passes; p0 += 4) {
+          uint4 v[4];
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) v[k] = live ? *reinterpret_cast<const uint4*>(src + (c + k) * 8) : make_uint4(0u, 0u, 0u, 0u);
+          for (int k = 0; k < 4; ++k) {
+            const int qr = (p0 + k) * RP + (int)threadIdx.x / PQ, qn = (g.row0 + qr) / A.G, qh = g.kvh * A.G + (g.row0 + qr) - qn * A.G;
+            v[k] = qr < g.rows ? *reinterpret_cast<const uint4*>((const bf16*)A.a.q + (long long)(g.s.n0 + qn) * A.a.q_row + (long long)qh * A.a.q_head + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) st_shared16(dst + sw_off(r, c + k), v[k].x ^ qsign, v[k].y ^ qsign, v[k].z ^ qsign, v[k].w ^ qsign);
+          for (int k = 0; k < 4; ++k) {
+            const int qr = (p0 + k) * RP + (int)threadIdx.x / PQ;
+            uint4 y = make_uint4(v[k].x ^ qsign, v[k].y ^ qsign, v[k].z ^ qsign, v[k].w ^ qsign);
+            if (CODE != PCPB_BF16) {                            // q in f16, scaled by a power of two per row
+              uint32_t top = top_abs2(top_abs2(top_abs2(top_abs2(0u, y.x), y.y), y.z), y.w);
+#pragma unroll
+              for (int o = PQ / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const int e = exp15(top);
+              const float up = pow2(e);
+              y = make_uint4(bf16x2_to_f16x2(y.x, up), bf16x2_to_f16x2(y.y, up), bf16x2_to_f16x2(y.z, up), bf16x2_to_f16x2(y.w, up));
+              if (c == 0) qfac[qr] = pow2(-e);
+            }
+            st_shared16(sQ + (qr >> 7) * Cfg::TILE_BYTES + sw_off(qr & 127, c), y.x, y.y, y.z, y.w);
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(qfull);
@@ -925,6 +1014,8 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
 #pragma unroll 1
         for (int i = live ? node : -1; i >= 0; i = par[i]) anc[256 * (i >> 5)] |= 1u << (i & 31);
       }
+      // factor of the row's scores (codes: the keys' factors hold the scale); the first score tile comes after every thread's part of q
+      float rowf = zscale;
       float mref = -INFINITY;
       f32x2 l2 = pk2(0.f, 0.f);
       int done = 0;                                             // tiles of this stream in this segment
@@ -937,6 +1028,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         const uint4 valid = *reinterpret_cast<const uint4*>(info + 256);
         wait(sfull(x), sn & 1, &fail);
         tc_fence_after();
+        if (CODE != PCPB_BF16) rowf = qfac[tr];
         if (warp_live) {
           // The reference maximum moves (rarely): outputs, sums and the tile's weights so far (columns below 32 c) are scaled down.
           auto raise = [&](float top, int c) {
@@ -987,14 +1079,14 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
             }
             for (;;) {
               const float ref = mref == -INFINITY ? 0.f : mref;
-              const f32x2 nref = pk2(-ref, -ref), zs = pk2(zscale, zscale);
+              const f32x2 nref = pk2(-ref, -ref), zs = pk2(rowf, rowf);
               f32x2 s0 = pk2(0.f, 0.f), s1 = s0;
               float m0 = z[0], m1 = z[1];
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
                 f32x2 d0 = pk2(z[j], z[j + 1]), d1 = pk2(z[j + 2], z[j + 3]);
-                d0 = CODE == PCPB_BF16 ? fma2(d0, zs, nref) : add2(d0, nref);
-                d1 = CODE == PCPB_BF16 ? fma2(d1, zs, nref) : add2(d1, nref);
+                d0 = fma2(d0, zs, nref);
+                d1 = fma2(d1, zs, nref);
                 float e0, e1, e2, e3;
                 un2(d0, e0, e1); un2(d1, e2, e3);
                 m0 = max3(m0, z[j], z[j + 1]); m1 = max3(m1, z[j + 2], z[j + 3]);
@@ -1007,8 +1099,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
                 }
                 p[j / 2] = pack2(e0, e1); p[j / 2 + 1] = pack2(e2, e3);
               }
-              top = fmaxf(m0, m1);
-              if (CODE == PCPB_BF16) top *= zscale;
+              top = fmaxf(m0, m1) * rowf;
               sum = add2(s0, s1);
               if (!__any_sync(0xffffffffu, top > mref + 8.f || (mref == -INFINITY && top > -INFINITY))) break;
               raise(top, c);

@@ -1,5 +1,6 @@
 // Shared by the decode operators (kv_cache.cu, tree_attn.cu, verify.cu): argument checks on the host, lookups on the device.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdint.h>
@@ -21,6 +22,29 @@ inline int op_fail(char* err, size_t cap, int code, const char* fmt, ...) {
   return code;
 }
 
+// Driver entry point of the pointer query, resolved at run time (no link-time dependency on libcuda): one call for both attributes takes
+// a third of cudaPointerGetAttributes, and a small operator has a dozen pointers.
+typedef CUresult (*PointerQueryFn)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+inline PointerQueryFn pointer_query() {
+  static PointerQueryFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuPointerGetAttributes", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (PointerQueryFn)p : nullptr;
+  }();
+  return fn;
+}
+// Multiprocessors of a device, asked for once.
+inline int sm_count(int dev) {
+  static int known[64] = {};
+  if (dev < 0 || dev >= 64) return 148;
+  if (!known[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { cudaGetLastError(); return 148; }
+    known[dev] = n;
+  }
+  return known[dev];
+}
+
 // The device all pointers of a call live on becomes the current one for the call.
 struct OpDevice {
   char* err;
@@ -30,17 +54,16 @@ struct OpDevice {
   // `what` names the argument in the message; NULL is accepted (optional arguments)
   void on(const void* p, const char* what) {
     if (!p || rc) return;
-    cudaPointerAttributes a;
-    const cudaError_t e = cudaPointerGetAttributes(&a, p);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      rc = op_fail(err, cap, PCPB_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    } else if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) {
-      rc = op_fail(err, cap, PCPB_E_INVALID, "%s is not device memory", what);
-    } else if (a.type == cudaMemoryTypeDevice) {
-      if (dev < 0) dev = a.device;
-      if (a.device != dev) rc = op_fail(err, cap, PCPB_E_INVALID, "%s lives on device %d, the call's other arguments on device %d", what, a.device, dev);
-    }
+    const PointerQueryFn query = pointer_query();
+    unsigned type = 0;
+    int where = -1;
+    CUpointer_attribute which[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+    void* out[2] = {&type, &where};
+    const CUresult e = query ? query(2, which, out, (CUdeviceptr)p) : CUDA_ERROR_NOT_INITIALIZED;
+    if (e != CUDA_SUCCESS) rc = op_fail(err, cap, PCPB_E_CUDA, "%s: no CUDA device, or the driver refused the address (%d)", what, (int)e);
+    else if (type != CU_MEMORYTYPE_DEVICE && type != CU_MEMORYTYPE_UNIFIED) rc = op_fail(err, cap, PCPB_E_INVALID, "%s is not device memory", what);
+    else if (dev < 0) dev = where;
+    else if (where != dev) rc = op_fail(err, cap, PCPB_E_INVALID, "%s lives on device %d, the call's other arguments on device %d", what, where, dev);
   }
   int enter() {
     if (rc) return rc;

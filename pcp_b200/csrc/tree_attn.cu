@@ -1226,9 +1226,15 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
-int sm_count(int dev) {
-  int n = 0;
-  return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+// The attribute of a kernel on the current device, set once.
+template <typename K> cudaError_t allow_smem(K kern, bool (&done)[64], size_t bytes) {
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
 }
 struct Layout { size_t plan, ml, o, bytes; };
 Layout layout(const pcpb_kv_cache& c, int blocks, int rows_tile) {
@@ -1262,14 +1268,17 @@ template <int HD, int ROWS> cudaError_t launch_join(cudaStream_t st, const AttnA
 }
 template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnArgs& A, int blocks) {
   const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
-  cudaError_t e = cudaFuncSetAttribute(k_tree_rows<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static bool done[64] = {};
+  const size_t most = (MAX_BATCH + 1) * 8 + 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
+  cudaError_t e = allow_smem(k_tree_rows<HD, CODE>, done, most);
   if (e != cudaSuccess) return e;
   k_tree_rows<HD, CODE><<<blocks, Frag<HD, CODE>::WARPS * 32, smem, st>>>(A);
   e = cudaGetLastError();
   return e == cudaSuccess ? launch_join<HD, RW>(st, A, blocks) : e;
 }
 template <int HD, int CODE> cudaError_t launch_tc(cudaStream_t st, const AttnArgs& A, int blocks) {
-  cudaError_t e = cudaFuncSetAttribute(k_tree_tc<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HD>::BYTES);
+  static bool done[64] = {};
+  cudaError_t e = allow_smem(k_tree_tc<HD, CODE>, done, TcCfg<HD>::BYTES);
   if (e != cudaSuccess) return e;
   k_tree_tc<HD, CODE><<<blocks, TC_THREADS, TcCfg<HD>::BYTES, st>>>(A);
   e = cudaGetLastError();

@@ -409,7 +409,13 @@ template <typename T, bool GREEDY> cudaError_t launch(cudaStream_t st, const Ver
   int cl = 1;
   while (cl < MAX_CL && pieces > cl * 512ll) cl *= 2;
   if (cl > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static bool done[64] = {};
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev])) {
+      e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    }
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

@@ -15,6 +15,7 @@ call enqueues and returns.  A decoding step with drafts:
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 from .backend import BF16, F32, BackendError, E_INVALID, load_library
 
@@ -84,15 +85,16 @@ def _dtype(t):
     return name
 
 
-def _vector(t, what, dtype, n=None):
-    """Address of a contiguous tensor of one type (None stays None)."""
+def _vector(t, what, dtype, n=0):
+    """Address of a contiguous tensor of one type with at least n values (None stays None)."""
     if t is None:
         return None
-    if _dtype(t) != dtype:
+    d = t.dtype
+    if (_DTYPES.get(d) or _dtype(t)) != dtype:
         _refuse(f"{what} must be {dtype}, not {_dtype(t)}")
     if not t.is_contiguous():
         _refuse(f"{what} must be contiguous")
-    if n is not None and t.numel() < n:
+    if t.numel() < n:
         _refuse(f"{what} holds {t.numel()} values, {n} are needed")
     return t.data_ptr()
 
@@ -100,13 +102,15 @@ def _vector(t, what, dtype, n=None):
 def _rows(t, what, dtypes, heads, width):
     """(address, row stride, head stride) of a tensor [rows][heads][width] whose last dimension is dense."""
     shape, stride = t.shape, t.stride()
-    if _dtype(t) not in dtypes:
+    d = t.dtype
+    if (_DTYPES.get(d) or _dtype(t)) not in dtypes:
         _refuse(f"{what} must be {' or '.join(dtypes)}, not {_dtype(t)}")
     if len(shape) != 3 or shape[2] != width or (heads is not None and shape[1] != heads):
         _refuse(f"{what} must be [rows][{'heads' if heads is None else heads}][{width}], not {tuple(shape)}")
-    if stride[2] != 1:
+    r, h, e = stride
+    if e != 1:
         _refuse(f"the last dimension of {what} must be dense")
-    return t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
+    return t.data_ptr(), r if shape[0] > 1 else 0, h if shape[1] > 1 else 0
 
 
 _CODES = {"bfloat16": BF16, "int8": I8, "float8_e4m3fn": E4M3}
@@ -143,11 +147,21 @@ class KvCache:
         self._keep = (k, v, k_scale, v_scale, block_table)
 
 
+class _Err(threading.local):
+    """Room for the reason of a refusal, one per thread."""
+
+    def __init__(self):
+        self.buf = C.create_string_buffer(_ERR_CAP)
+
+
+_err = _Err()
+
+
 def _call(fn, stream, *args):
-    err = C.create_string_buffer(_ERR_CAP)
-    rc = fn(stream, *args, err, _ERR_CAP)
+    buf = _err.buf
+    rc = fn(stream, *args, buf, _ERR_CAP)
     if rc:
-        raise BackendError(rc, err.value.decode())
+        raise BackendError(rc, buf.value.decode())
 
 
 def _kv_rows(fn, cache, k, v, cu_rows, pos0, n_entries, index, status, stream):

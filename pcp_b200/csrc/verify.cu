@@ -27,6 +27,7 @@ namespace cg = cooperative_groups;
 constexpr int VW = 8, VT = 32 * (VW + 1);          // warps that read rows, threads of a block: one more warp looks after the children
 constexpr int MAX_CL = 16;                         // blocks of a cluster
 constexpr int MAX_N = PCPB_TREE_MAX_NODES;
+constexpr int KEEP = 10;                           // a lane's first pieces of the last token's row, whose sums are kept for the search
 constexpr int AHEAD_N = 64;                        // most nodes whose rows are all read ahead of the walk
 constexpr double AHEAD_BYTES = 32e6;
 
@@ -165,6 +166,8 @@ struct Shared {
   float kz[MAX_N], kq[MAX_N];
   uint8_t gone[MAX_N];                             // the child's token has no weight left
   int nkid;
+  int refused[MAX_N];                              // those tokens, for the last token's sum
+  double kept[VW][KEEP][32];
 };
 
 // What is left of a row's distribution: weights max(e_i - aS q_i, 0) with e_i = exp((z_i - max) / T), the refused tokens' weights 0.
@@ -180,17 +183,18 @@ template <typename T> struct Left {
     if (q) { w -= aS * (double)__ldg(q + i); return w > 0.0 ? w : 0.0; }
     return w;
   }
-  // weights of piece j
-  __device__ __forceinline__ void weights(int j, const Shared& sh, double (&w)[Pieces<T>::E]) const {
+  // weights of piece j from its raw bits
+  __device__ __forceinline__ void weights(int j, const uint4& raw, const Shared& sh, double (&w)[Pieces<T>::E]) const {
     constexpr int E = Pieces<T>::E;
     float f[E];
-    P.load(j, f);
+    P.values(j, raw, f);
     const int i0 = P.first(j);
 #pragma unroll
     for (int i = 0; i < E; ++i) w[i] = weight(f[i], i0 + i, sh);
+#pragma unroll 1
     for (int k = 0; k < nref; ++k) {
-      const long long d = sh.token[sh.kid[k]] - i0;
-      if (sh.gone[k] && d >= 0 && d < E)
+      const unsigned d = (unsigned)(sh.refused[k] - i0);
+      if (d < (unsigned)E)
 #pragma unroll
         for (int i = 0; i < E; ++i) if (i == (int)d) w[i] = 0.0;
     }
@@ -198,7 +202,8 @@ template <typename T> struct Left {
 };
 
 template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verify(const __grid_constant__ VerifyArgs A) {
-  __shared__ Shared sh;
+  extern __shared__ __align__(16) uint8_t verify_smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(verify_smem);
   cg::cluster_group cl = cg::this_cluster();
   cl.barrier_arrive();                                          // waited for before the first write into another block
   const pcpb_verify& v = A.v;
@@ -330,21 +335,29 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verif
     double S = (double)st.s, a = 0.0, a0 = 0.0, D = 1.0;
     bool sure = false;                                          // S is a 64-bit sum
     int which;
-    constexpr int KEEP = 10;                                    // a lane's first pieces, whose sums are kept for the search below
-    double kept[KEEP];
     auto sum_left = [&]() {                                     // sum of the weights that are left
       double x = 0.0;
       left.aS = a * S;
+      uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;           // two pieces at a time, the next two on their way
+      if (j0 + lane < j1) w0 = P.raw(j0 + lane);
+      if (j0 + lane + 32 < j1) w1 = P.raw(j0 + lane + 32);
+#pragma unroll 1
+      for (int j = j0 + lane, q = 0; j < j1; j += 64, q += 2) {
+        const uint4 c0 = w0, c1 = w1;
+        if (j + 64 < j1) w0 = P.raw(j + 64);
+        if (j + 96 < j1) w1 = P.raw(j + 96);
+        double u[Pieces<T>::E], y[Pieces<T>::E];
+        left.weights(j, c0, sh, u);
+        if (j + 32 < j1) left.weights(j + 32, c1, sh, y);
+        else
 #pragma unroll
-      for (int q = 0; q < KEEP; ++q) kept[q] = 0.0;
-      for (int j = j0 + lane, q = 0; j < j1; j += 32, ++q) {
-        double w[Pieces<T>::E], y = 0.0;
-        left.weights(j, sh, w);
+          for (int i = 0; i < Pieces<T>::E; ++i) y[i] = 0.0;
 #pragma unroll
-        for (int i = 0; i < Pieces<T>::E; ++i) y += w[i];
+        for (int i = Pieces<T>::E / 2; i > 0; i >>= 1)
 #pragma unroll
-        for (int k = 0; k < KEEP; ++k) kept[k] = q == k ? y : kept[k];
-        x += y;
+          for (int k = 0; k < i; ++k) { u[k] += u[k + i]; y[k] += y[k + i]; }
+        if (q < KEEP) { sh.kept[warp][q][lane] = u[0]; sh.kept[warp][q + 1][lane] = y[0]; }
+        x += u[0] + y[0];
       }
       return exchange(x, &which);
     };
@@ -390,7 +403,12 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verif
     if (taken < 0 && !GREEDY && choice) {                       // the last token
       if (qrow && !sure && a > 0.0) make_sure();
       __syncthreads();
-      left.nref = qrow ? 0 : nkid;
+      int nref = 0;
+      if (!qrow)
+        for (int k = 0; k < nkid; ++k)
+          if (sh.gone[k]) { if (tid == 0) sh.refused[nref] = (int)sh.token[sh.kid[k]]; ++nref; }
+      __syncthreads();
+      left.nref = nref;
       double total = sum_left();
       if (!(total > 0.0) && (a > 0.0 || left.nref)) { a = a0; left.nref = 0; total = sum_left(); }
       // the last segment that begins at or before the goal and is not empty
@@ -418,14 +436,15 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verif
         for (int base = j0, q = 0; base < j1; base += 32, ++q) {
           const int j = base + lane;
           double x = 0.0;
-          if (q < KEEP) {
+          if (j < j1) {
+            if (q < KEEP) {
+              x = sh.kept[warp][q][lane];
+            } else {
+              double w[Pieces<T>::E];
+              left.weights(j, P.raw(j), sh, w);
 #pragma unroll
-            for (int k = 0; k < KEEP; ++k) x = q == k ? kept[k] : x;
-          } else if (j < j1) {
-            double w[Pieces<T>::E];
-            left.weights(j, sh, w);
-#pragma unroll
-            for (int i = 0; i < Pieces<T>::E; ++i) x += w[i];
+              for (int i = 0; i < Pieces<T>::E; ++i) x += w[i];
+            }
           }
           double inc = x;
 #pragma unroll
@@ -438,7 +457,7 @@ template <typename T, bool GREEDY> __global__ void __launch_bounds__(VT) k_verif
         int hit = -1, lastpos = -1;
         if (piece >= 0) {
           double w[Pieces<T>::E], r = begin;
-          left.weights(piece, sh, w);
+          left.weights(piece, P.raw(piece), sh, w);
 #pragma unroll
           for (int i = 0; i < Pieces<T>::E; ++i) {
             r += w[i];
@@ -470,18 +489,17 @@ template <typename T, bool GREEDY> cudaError_t launch(cudaStream_t st, const Ver
   const long long pieces = ((long long)A.v.vocab * (long long)sizeof(T) + 15) / 16;
   int cl = 1;
   while (cl < MAX_CL && pieces > cl * 512ll && (cl < 2 || 2ll * cl * A.v.batch <= (cl < 8 ? 2 * 148 : 148))) cl *= 2;
-  if (cl > 8) {
-    static bool done[64] = {};
-    int dev = -1;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev])) {
-      e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
-    }
-    if (e != cudaSuccess) return e;
+  static bool done[64] = {};                       // attributes of the kernel on a device, set once
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev])) {
+    e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_verify<T, GREEDY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
   }
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)A.v.batch * cl); cfg.blockDim = dim3(VT); cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)A.v.batch * cl); cfg.blockDim = dim3(VT); cfg.dynamicSmemBytes = sizeof(Shared); cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cl; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;

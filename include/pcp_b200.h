@@ -364,6 +364,9 @@ typedef struct pcpb_rollout_cfg {
  * Hugging Face model): embed, per layer q k v o q_norm k_norm gate up down input_ln post_ln, norm, lm_head. */
 long long pcpb_rollout_num_params(const pcpb_rollout_cfg* cfg);
 int pcpb_rollout_create(int device_ordinal, const pcpb_rollout_cfg* cfg, pcpb_rollout** out);
+/* The same engine with the cache's element type: PCPB_BF16 (pcpb_rollout_create), PCPB_E4M3 or PCPB_I8, which halve the cache.
+ * Prompt tokens attend each other's keys and values before they are quantised; generated tokens attend the quantised ones. */
+int pcpb_rollout_create_cached(int device_ordinal, const pcpb_rollout_cfg* cfg, int cache_dtype, pcpb_rollout** out);
 void pcpb_rollout_destroy(pcpb_rollout* r);
 const char* pcpb_rollout_last_error(const pcpb_rollout* r);
 /* GenerationEngine.ensureDeviceWeights (generation_engine.zig:80-122): the weight blob, tensor after tensor, PCPB_F32

@@ -28,6 +28,7 @@ DTYPE_SIZE = {F32: 4, F64: 8, F16: 2, BF16: 2, I32: 4, I64: 8, BOOL: 1}
 _NP_DTYPE = {F32: np.float32, F64: np.float64, F16: np.float16, BF16: np.uint16, I32: np.int32, I64: np.int64,
              BOOL: np.uint8}
 IPC_HANDLE_BYTES = 64
+CACHE_DTYPES = {"bf16": BF16, "i8": 16, "e4m3": 17}      # of the rollout engine's KV cache
 
 E_INVALID, E_CUDA, E_ARTIFACT, E_FUNCTION, E_CHUNK_TOO_SMALL, E_CHUNK_EXHAUSTED, E_STATE, E_TOO_LARGE = range(1, 9)
 
@@ -46,7 +47,7 @@ EXPORTS = [
     "pcpb_stream_merge", "pcpb_prng_seed", "pcpb_prng_next", "pcpb_prng_uint_at_most", "pcpb_random_window_starts",
     "pcpb_random_get_batch", "pcpb_char_tokenizer_build", "pcpb_char_encode", "pcpb_char_decode",
     "pcpb_init_master_elems", "pcpb_init_master", "pcpb_worker_write_state", "pcpb_worker_set_sampling",
-    "pcpb_adjoint_status", "pcpb_rollout_num_params", "pcpb_rollout_create", "pcpb_rollout_destroy", "pcpb_rollout_last_error",
+    "pcpb_adjoint_status", "pcpb_rollout_num_params", "pcpb_rollout_create", "pcpb_rollout_create_cached", "pcpb_rollout_destroy", "pcpb_rollout_last_error",
     "pcpb_rollout_load_weights", "pcpb_rollout_random_weights", "pcpb_rollout_generate", "pcpb_rollout_read_logits",
     "pcpb_rollout_launch_count", "pcpb_op_kv_write", "pcpb_op_kv_read", "pcpb_op_tree_attention",
     "pcpb_op_tree_attention_workspace", "pcpb_op_verify_drafts",
@@ -173,6 +174,8 @@ def load_library(path: str | None = None):
         rc = C.POINTER(RolloutCfg)
         lib.pcpb_rollout_num_params.argtypes = [rc]; lib.pcpb_rollout_num_params.restype = C.c_longlong
         lib.pcpb_rollout_create.argtypes = [i, rc, C.POINTER(vp)]
+        if hasattr(lib, "pcpb_rollout_create_cached"):
+            lib.pcpb_rollout_create_cached.argtypes = [i, rc, i, C.POINTER(vp)]
         lib.pcpb_rollout_destroy.argtypes = [vp]; lib.pcpb_rollout_destroy.restype = None
         lib.pcpb_rollout_last_error.argtypes = [vp]; lib.pcpb_rollout_last_error.restype = C.c_char_p
         lib.pcpb_rollout_load_weights.argtypes = [vp, vp, sz, i]
@@ -716,12 +719,18 @@ class Rollout:
     ensureDeviceWeights -> ensure_device_weights, generateRollout -> generate_rollout."""
 
     def __init__(self, device_id: int, vocab, d_model, n_layer, n_head, n_kv_head, head_dim, d_ff, max_seq, max_batch=16,
-                 max_prompt=None, page_tokens=16, rope_theta=1e6, rms_eps=1e-6):
+                 max_prompt=None, page_tokens=16, rope_theta=1e6, rms_eps=1e-6, cache="bf16"):
+        """cache: element type of the KV cache, "bf16", "e4m3" or "i8" (see include/pcp_b200.h)."""
         self._lib = load_library()
+        if cache not in CACHE_DTYPES:
+            raise ValueError(f"cache must be one of {', '.join(CACHE_DTYPES)}")
         self.cfg = RolloutCfg(vocab, d_model, n_layer, n_head, n_kv_head, head_dim, d_ff, max_seq, page_tokens, max_batch,
                               max_prompt if max_prompt is not None else max_seq, rope_theta, rms_eps)
         h = C.c_void_p()
-        rc = self._lib.pcpb_rollout_create(device_id, C.byref(self.cfg), C.byref(h))
+        if cache == "bf16":
+            rc = self._lib.pcpb_rollout_create(device_id, C.byref(self.cfg), C.byref(h))
+        else:
+            rc = self._lib.pcpb_rollout_create_cached(device_id, C.byref(self.cfg), CACHE_DTYPES[cache], C.byref(h))
         self._h = h
         if rc:
             msg = self._lib.pcpb_rollout_last_error(h).decode() if h else "allocation failed"

@@ -16,6 +16,10 @@
 //   KV cache    pages of PAGE tokens: kpages / vpages [layer][page][kv_head][PAGE][head_dim] bf16; block_table
 //               [sequence][logical page] -> physical page.  Pages are handed out round-robin over the sequences, so a
 //               sequence's pages are not contiguous.
+//               An 8-bit cache (pcpb_rollout_create_cached) holds codes and scales instead, through the decode operators: a layer's
+//               new rows pass through one layer of bf16 pages, are gathered from there (pcpb_op_kv_read), serve the step's attention
+//               and are quantised into the layer's cache (pcpb_op_kv_write).  Prompt rows attend each other before they are
+//               quantised, as ever; decode rows attend the codes (pcpb_op_tree_attention, a tree of one node with a zero slot).
 //   decode      activations of the <= 16 sequences in 16-row buffers; every decode step is one CUDA graph launch
 //               (token ids and positions live on the device, so the graph does not change from step to step).
 //
@@ -677,6 +681,14 @@ struct pcpb_rollout {
   bf16 *kpages = nullptr, *vpages = nullptr, *cosT = nullptr, *sinT = nullptr;
   bf16 *sqk = nullptr, *sqv = nullptr;   // prefill staging for the tensor-core attention: [rows, hq + hk] (q | shifted k), [rows, hq + 2 hk] (v part: shifted v)
   float *att_m = nullptr, *att_l = nullptr;
+  // 8-bit cache: codes and scales of all layers (kpages / vpages then hold one layer's rows on their way), gathered rows, index arrays
+  int cache_dtype = PCPB_BF16, seqs = 0;      // seqs: sequences of the pass being enqueued
+  uint8_t *k8 = nullptr, *v8 = nullptr;
+  float *k8_scale = nullptr, *v8_scale = nullptr;
+  bf16 *rows_k = nullptr, *rows_v = nullptr;
+  int *cu_prompt = nullptr, *cu_step = nullptr, *zeros = nullptr;
+  void* att_ws = nullptr;
+  size_t att_ws_bytes = 0;
   int *block_table = nullptr, *row_seq = nullptr, *row_pos = nullptr, *last_row = nullptr, *drow_seq = nullptr, *cur_pos = nullptr,
       *step = nullptr, *tc_err = nullptr;
   long long *row_tok = nullptr, *cur_tok = nullptr, *out_tok = nullptr;
@@ -851,6 +863,58 @@ int attention(pcpb_rollout* r, const bf16* q, const int* rs, const int* rp, int 
   return PCPB_OK;
 }
 
+// The decode operators on a layer's caches: `codes` is the 8-bit cache, else the layer of bf16 pages its rows pass through.
+pcpb_kv_cache kv_cache_of(const pcpb_rollout* r, int layer, bool codes) {
+  const pcpb_rollout_cfg& c = r->cfg;
+  pcpb_kv_cache k{};
+  const size_t rows = (size_t)layer * r->n_pages * c.n_kv_head * c.page_tokens;
+  k.k = codes ? (void*)(r->k8 + rows * c.head_dim) : (void*)r->kpages;
+  k.v = codes ? (void*)(r->v8 + rows * c.head_dim) : (void*)r->vpages;
+  if (codes) { k.k_scale = r->k8_scale + rows; k.v_scale = r->v8_scale + rows; }
+  k.block_table = r->block_table;
+  k.dtype = codes ? r->cache_dtype : PCPB_BF16;
+  k.n_pages = r->n_pages; k.n_kv_head = c.n_kv_head; k.head_dim = c.head_dim; k.page_tokens = c.page_tokens;
+  k.batch = r->seqs; k.max_pages = r->max_pages;
+  return k;
+}
+#define ROP(r, call)                                                \
+  do {                                                              \
+    char e__[256] = "";                                             \
+    const int rc__ = (call);                                        \
+    if (rc__) return rfail((r), rc__, e__);                         \
+  } while (0)
+// The rows of a pass (M of them, sequence by sequence) out of the bf16 pages, the step's attention over the codes, the rows into the codes
+int gather_rows(pcpb_rollout* r, int M, const int* cu, const int* pos0, pcpb_kv_rows* rows) {
+  const pcpb_rollout_cfg& c = r->cfg;
+  const pcpb_kv_cache pages = kv_cache_of(r, 0, false);
+  *rows = pcpb_kv_rows{};
+  rows->k = r->rows_k; rows->v = r->rows_v;
+  rows->k_row = rows->v_row = r->hk; rows->k_head = rows->v_head = c.head_dim;
+  rows->cu_rows = cu; rows->pos0 = pos0; rows->dtype = PCPB_BF16; rows->n_rows = M; rows->n_entries = M;
+  r->launches += 1;
+  ROP(r, pcpb_op_kv_read(r->stream, &pages, rows, nullptr, e__, sizeof e__));
+  return PCPB_OK;
+}
+int attend_codes(pcpb_rollout* r, int layer, int B, const bf16* q, const int* cur_pos, bf16* out) {
+  const pcpb_rollout_cfg& c = r->cfg;
+  const pcpb_kv_cache cache = kv_cache_of(r, layer, true);
+  pcpb_tree_attn a{};
+  a.q = q; a.k = r->rows_k; a.v = r->rows_v; a.out = out;
+  a.q_row = a.out_row = r->hq; a.k_row = a.v_row = r->hk;
+  a.q_head = a.k_head = a.v_head = a.out_head = c.head_dim;
+  a.cu_nodes = r->cu_step; a.ctx_len = cur_pos; a.workspace = r->att_ws; a.workspace_bytes = r->att_ws_bytes;
+  a.n_rows = B; a.n_head = c.n_head; a.max_nodes = 1; a.null_self = 1; a.scale = 1.f;          // q comes divided by sqrt(head_dim)
+  r->launches += 2;
+  ROP(r, pcpb_op_tree_attention(r->stream, &cache, &a, nullptr, e__, sizeof e__));
+  return PCPB_OK;
+}
+int store_rows(pcpb_rollout* r, int layer, const pcpb_kv_rows* rows) {
+  const pcpb_kv_cache cache = kv_cache_of(r, layer, true);
+  r->launches += 1;
+  ROP(r, pcpb_op_kv_write(r->stream, &cache, rows, nullptr, e__, sizeof e__));
+  return PCPB_OK;
+}
+
 // One pass over the layers for M token rows.  decode: the 16-row buffers and the GEMV kernels; else prefill.
 // tc_T > 0 (prefill only): every sequence has tc_T prompt rows, a multiple of 128, and head_dim is 128: the attention runs
 // on the tcgen05 kernel over staged q / shifted k, v buffers instead of the row kernel.
@@ -879,7 +943,7 @@ int layers(pcpb_rollout* r, bool decode, int M, const int* rs, const int* rp, in
     if (decode) { if ((rc = gemv(r, GV_STORE, x, W(r, p0), nullptr, nqkv, d, qkv, nqkv, nullptr))) return rc; }
     else if ((rc = big_gemm(r, x, W(r, p0), qkv, Mp, nqkv, d, EPI_STORE, nullptr))) return rc;
     const long long warps = (long long)M * (c.n_head + 2 * c.n_kv_head);
-    const size_t layer_pages = (size_t)l * r->n_pages * c.n_kv_head * c.page_tokens * c.head_dim;
+    const size_t layer_pages = r->k8 ? 0 : (size_t)l * r->n_pages * c.n_kv_head * c.page_tokens * c.head_dim;
     bf16 *kp = r->kpages + layer_pages, *vp = r->vpages + layer_pages;
     r->launches += 1;
     RCK(r, klaunch(r, k_qknorm_rope_cache, dim3((unsigned)((warps * 32 + 255) / 256)), dim3(256), 0, (const bf16*)qkv, W(r, p0 + 4),
@@ -887,13 +951,18 @@ int layers(pcpb_rollout* r, bool decode, int M, const int* rs, const int* rp, in
                    (const int*)r->block_table, r->max_pages, c.page_tokens, kp, vp, q, tc_attn ? r->sqk : (bf16*)nullptr,
                    tc_attn ? r->sqv : (bf16*)nullptr, tc_T));
     // the row's own key / value are in the cache now, but its attention reads only the slots below its position
-    if (tc_attn) {
+    pcpb_kv_rows rows{};
+    if (r->k8 && (rc = gather_rows(r, M, decode ? r->cu_step : r->cu_prompt, decode ? rp : r->zeros, &rows))) return rc;
+    if (r->k8 && decode) {
+      if ((rc = attend_codes(r, l, M, q, rp, att))) return rc;
+    } else if (tc_attn) {
       FlashArgs fa{};
       fa.qkn = r->sqk; fa.qkv = r->sqv; fa.o = att; fa.mrow = r->att_m; fa.lrow = r->att_l;
       fa.B = M / tc_T; fa.T = tc_T; fa.H = c.n_head; fa.Hkv = c.n_kv_head; fa.hd = c.head_dim; fa.scale = 1.f; fa.no_guard = 1;
       r->launches += 1;
       RCK(r, launch_attn_tc_fwd(st, fa, r->tc_err));
     } else if ((rc = attention(r, q, rs, rp, M, kp, vp, att))) return rc;
+    if (r->k8 && (rc = store_rows(r, l, &rows))) return rc;
     if (decode) { if ((rc = gemv(r, GV_RESID, att, W(r, p0 + 3), nullptr, d, hq, h2, d, h))) return rc; }
     else if ((rc = big_gemm(r, att, W(r, p0 + 3), h2, Mp, d, hq, EPI_RESID, h))) return rc;
     r->launches += 1;
@@ -965,11 +1034,17 @@ long long pcpb_rollout_num_params(const pcpb_rollout_cfg* c) {
 }
 
 int pcpb_rollout_create(int device, const pcpb_rollout_cfg* cfg, pcpb_rollout** out) {
+  return pcpb_rollout_create_cached(device, cfg, PCPB_BF16, out);
+}
+
+int pcpb_rollout_create_cached(int device, const pcpb_rollout_cfg* cfg, int cache_dtype, pcpb_rollout** out) {
   if (!out || !cfg) return PCPB_E_INVALID;
   pcpb_rollout* r = new pcpb_rollout();
   *out = r;                                            // returned even on failure so that the message can be read
   r->device = device; r->cfg = *cfg;
   const pcpb_rollout_cfg& c = r->cfg;
+  if (cache_dtype != PCPB_BF16 && cache_dtype != PCPB_E4M3 && cache_dtype != PCPB_I8) return rfail(r, PCPB_E_INVALID, "cache dtype must be bf16, e4m3 or i8");
+  r->cache_dtype = cache_dtype;
   int ndev = 0;
   if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) return rfail(r, PCPB_E_CUDA, "no CUDA device");
   if (device < 0 || device >= ndev) return rfail(r, PCPB_E_INVALID, "device ordinal out of range");
@@ -1021,7 +1096,28 @@ int pcpb_rollout_create(int device, const pcpb_rollout_cfg* cfg, pcpb_rollout** 
   RA(r, r->dq, ROWS * (size_t)r->hq * 2); RA(r, r->datt, ROWS * (size_t)r->hq * 2); RA(r, r->dact, ROWS * f * 2);
   RA(r, r->logits, ROWS * (size_t)c.vocab * 2);
   const size_t cache = (size_t)c.n_layer * r->n_pages * c.n_kv_head * c.page_tokens * c.head_dim;
-  RA(r, r->kpages, cache * 2); RA(r, r->vpages, cache * 2);
+  if (cache_dtype == PCPB_BF16) {
+    RA(r, r->kpages, cache * 2); RA(r, r->vpages, cache * 2);
+  } else {
+    const size_t one = cache / c.n_layer, most = std::max(MR, (size_t)ROWS);
+    RA(r, r->kpages, one * 2); RA(r, r->vpages, one * 2);
+    RA(r, r->k8, cache); RA(r, r->v8, cache);
+    RA(r, r->k8_scale, cache / c.head_dim * 4); RA(r, r->v8_scale, cache / c.head_dim * 4);
+    RA(r, r->rows_k, most * r->hk * 2); RA(r, r->rows_v, most * r->hk * 2);
+    RA(r, r->cu_prompt, (ROWS + 1) * 4); RA(r, r->cu_step, (ROWS + 1) * 4); RA(r, r->zeros, ROWS * 4);
+    int step[ROWS + 1];
+    for (int i = 0; i <= ROWS; ++i) step[i] = i;
+    RCK(r, cudaMemcpy(r->cu_step, step, sizeof step, cudaMemcpyHostToDevice));
+    RCK(r, cudaMemset(r->zeros, 0, ROWS * 4));
+    pcpb_kv_cache k{};                                    // the geometry alone decides the size; the addresses are set per layer
+    char e[256] = "";
+    r->seqs = c.max_batch;
+    k = kv_cache_of(r, 0, true);
+    k.block_table = r->cu_step;                           // (allocated below; any address will do here)
+    r->att_ws_bytes = pcpb_op_tree_attention_workspace(device, &k, c.n_head, 1, e, sizeof e);
+    if (!r->att_ws_bytes) return rfail(r, PCPB_E_INVALID, e);
+    RA(r, r->att_ws, r->att_ws_bytes);
+  }
   RA(r, r->cosT, (size_t)c.max_seq * c.head_dim * 2); RA(r, r->sinT, (size_t)c.max_seq * c.head_dim * 2);
   RA(r, r->block_table, (size_t)c.max_batch * r->max_pages * 4);
   RA(r, r->row_seq, MR * 4); RA(r, r->row_pos, MR * 4); RA(r, r->row_tok, MR * 8); RA(r, r->last_row, ROWS * 4);
@@ -1173,6 +1269,12 @@ int pcpb_rollout_generate(pcpb_rollout* r, const int64_t* prompts, const int* pr
   RCK(r, cudaMemcpyAsync(r->last_row, last.data(), (size_t)batch * 4, cudaMemcpyHostToDevice, st));
   RCK(r, cudaMemcpyAsync(r->drow_seq, dseq.data(), ROWS * 4, cudaMemcpyHostToDevice, st));
   RCK(r, cudaMemcpyAsync(r->cur_pos, dpos.data(), ROWS * 4, cudaMemcpyHostToDevice, st));
+  if (r->k8) {
+    std::vector<int> cu(batch + 1, 0);
+    for (int b = 0; b < batch; ++b) cu[b + 1] = cu[b] + lens[b];
+    RCK(r, cudaMemcpyAsync(r->cu_prompt, cu.data(), cu.size() * 4, cudaMemcpyHostToDevice, st));
+    r->seqs = batch;
+  }
   RCK(r, cudaMemsetAsync(r->step, 0, 4, st));
   RCK(r, cudaMemsetAsync(r->out_tok, 0, (size_t)ROWS * max_new_tokens * 8, st));
   // ---- prefill: all prompt tokens at once; the first new token comes from each sequence's last prompt row ----

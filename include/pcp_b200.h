@@ -411,7 +411,8 @@ long long pcpb_rollout_launch_count(const pcpb_rollout* r);
  * sequence b is row t % page_tokens of page block_table[b * max_pages + t / page_tokens].  dtype PCPB_BF16 holds the rows
  * as they are; PCPB_E4M3 and PCPB_I8 hold codes c and per row and head one f32 scale a, value a * c:
  *   a = max(largest magnitude of the row / Q, 2^-126), Q = 448 (e4m3) or 127 (i8);  c = x / a (f32) rounded to nearest even.
- * A row with an infinity or a NaN gets scale NaN, so that all of it reads back as NaN. */
+ * A row with an infinity or a NaN gets scale NaN, so that all of it reads back as NaN.  The codes are those pcpb_op_kv_write
+ * makes: e4m3's NaN code and -128 are not among them. */
 typedef struct pcpb_kv_cache {
   void *k, *v;
   float *k_scale, *v_scale;        /* [page][n_kv_head][page_tokens]; NULL for PCPB_BF16 */
@@ -434,7 +435,8 @@ typedef struct pcpb_kv_rows {
  * sequences whose block tables share the page, or an index list that names a page twice) leave either row or a mix of both
  * there. */
 int pcpb_op_kv_write(void* stream, const pcpb_kv_cache* cache, const pcpb_kv_rows* rows, int32_t* status, char* err, size_t err_cap);
-/* Reads rows of the cache back as values (a * c in f32, rounded once to rows->dtype).  Rows of bad pages become zero. */
+/* Reads rows of the cache back as values (a * c in f32, rounded once to rows->dtype).  Rows of bad pages become zero.  An index
+ * list that names a row twice leaves either entry's values or a mix there. */
 int pcpb_op_kv_read(void* stream, const pcpb_kv_cache* cache, const pcpb_kv_rows* rows, int32_t* status, char* err, size_t err_cap);
 
 /* Attention of the nodes of drafted trees over the cache (bf16 in and out, f32 softmax).  Sequence b has the nodes
@@ -446,7 +448,8 @@ int pcpb_op_kv_read(void* stream, const pcpb_kv_cache* cache, const pcpb_kv_rows
  * afterwards).  A single token per sequence is a tree of one node.  null_self = 1: a node's own slot counts as a zero key
  * and a zero value instead, the rule of the exported decode step (see pcpb_rollout above).
  * The weights are rounded to bf16 before they meet the values (their sum is not); keys and values of 8-bit caches enter
- * exactly, with their scales in f32 on the scores and the weights.  lse (optional) [n_rows][n_head] f32 receives the
+ * exactly, with their scales in f32 on the scores and the weights (against q, and the nodes' own keys, in f16 with a power of two
+ * per row: exact but for elements below 2^-29 of their row's largest, which are off by at most 2^-40 of it).  lse (optional) [n_rows][n_head] f32 receives the
  * natural logarithm of each row's sum of exponentials.  Rows of out and lse behind cu_nodes[batch] are left as they are. */
 #define PCPB_TREE_MAX_NODES 256
 #define PCPB_TREE_MAX_BATCH 1024

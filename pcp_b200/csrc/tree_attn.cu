@@ -569,10 +569,10 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
   const Seq s = seq_of(A, b);
   const int rows = s.n * A.G, RT = (rows + ROWS - 1) / ROWS, T = tiles_of(s.ctx) + tiles_of(s.n);
   const int item = blockIdx.y;
+  pdl_wait();                                                   // in every block: whatever comes after this kernel comes after the attention too
   if (item >= RT * A.c.n_kv_head) return;
   const int kvh = item / RT, row0 = item % RT * ROWS, r0 = blockIdx.z * 16;
   if (row0 + r0 >= rows) return;
-  pdl_wait();
   const Parts P = parts_of(A.plan[b] + (long long)item * T, T, tile_share(A.plan[A.c.batch], blocks));
   if (P.c0 == P.c1) return;
   for (int i = threadIdx.x; i < 16 * (HD / 4); i += blockDim.x) {

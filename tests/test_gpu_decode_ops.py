@@ -244,6 +244,10 @@ CASES = [
     (128, "bf16", 1, 1, 128, [256], [0], "chain"),
     (128, "bf16", 2, 1, 16, [256], [90], "tree"),
     (128, "e4m3", 5, 1, 16, [33], [3000], "tree"),
+    (128, "e4m3", 16, 1, 16, [1], [600], "chain"),
+    (128, "i8", 8, 1, 16, [1, 1], [2000, 31], "chain"),
+    (64, "i8", 2, 3, 16, [65, 64, 63], [128, 64, 192], "tree"),
+    (128, "bf16", 1, 2, 16, [129], [64], "roots"),
     (64, "bf16", 4, 1, 16, [2] * 50, [(37 * i) % 400 for i in range(50)], "chain"),
 ]
 
@@ -458,6 +462,71 @@ def test_side_stream_and_graph_replay():
     ops.tree_attention(*s["args"], **s["kw"])
     assert torch.equal(out[:14], out_r[:14])
     del graph
+
+
+def test_first_call_inside_a_capture_and_calls_without_nodes():
+    """A process whose first use of a kernel is a captured one; sequences that are all empty leave everything as it is."""
+    s = _attention_case(32, "i8", 3, 1, 8, [2, 3], [40, 9], "tree", lse=False)
+    want = s["out"].clone()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    v = _verify_case([3], 40, 0.0, "chain", False, dtype=torch.float32)
+    with torch.cuda.graph(graph, stream=side):
+        ops.tree_attention(*s["args"], **s["kw"], stream=side.cuda_stream)
+        ops.verify_drafts(*v["args"], **v["kw"], stream=side.cuda_stream)
+    s["out"][:5].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(s["out"], want)
+    del graph
+    none = list(s["args"])
+    none[5] = _i32([0, 0, 0])
+    for hd in (32, 128):
+        e = _attention_case(hd, "bf16", 4, 2, 16, [0, 0], [40, 9], "tree", lse=False)
+        assert e["status"] == 0 and (e["out"] == 3.0).all()
+    ops.tree_attention(*none, **s["kw"])
+    assert torch.equal(s["out"], want)
+
+
+def test_two_calls_at_once_share_the_inputs():
+    """Two streams, one cache and one set of inputs, two outputs and workspaces."""
+    for case in ((128, "e4m3", 4, 2, 16, [1, 1, 1], [3000, 2000, 50], "chain"), (128, "bf16", 4, 2, 16, [24, 9, 17], [900, 2000, 50], "tree")):
+        s = _attention_case(*case, lse=False)
+        cache, q, kn, vn, out, cu, par, ctx, most, ws = s["args"]
+        outs, spaces = [torch.full_like(out, 3.0) for _ in range(2)], [torch.empty_like(ws) for _ in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for i in range(2):
+                ops.tree_attention(cache, q, kn, vn, outs[i], cu, par, ctx, most, spaces[i], stream=streams[i].cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], out) and torch.equal(outs[1], out)
+
+
+@pytest.mark.parametrize("nodes", [[1], [40]])
+def test_offsets_pass_32_bits(nodes):
+    """Two pages more than 2^31 elements apart: the second one is written, attended and read back."""
+    hd, page, stride = 64, 16, (1 << 31) + 4096
+    big = [torch.zeros(stride + hd * page, dtype=torch.int8, device=DEV) for _ in range(2)]
+    k, v = (t.as_strided((2, 1, page, hd), (stride, page * hd, hd, 1)) for t in big)
+    ks, vs = (torch.zeros(2, 1, page, device=DEV) for _ in range(2))
+    bt = torch.tensor([[1, 0]], dtype=I32)
+    cache = ops.KvCache(k, v, bt.to(DEV), ks, vs)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(24, 2, hd, generator=g).to(torch.bfloat16).to(DEV)
+    ops.kv_write(cache, x[:, :1], x[:, 1:], _i32([0, 24]), _i32([0]), 24)
+    back = [torch.zeros(24, 1, hd, device=DEV) for _ in range(2)]
+    ops.kv_read(cache, back[0], back[1], _i32([0, 24]), _i32([0]), 24)
+    for i in range(2):
+        assert torch.equal(back[i].cpu(), ref.values(*ref.quantise(x[:, i:i + 1], "i8")).float())
+    n = nodes[0]
+    f = torch.randn(n, 3, hd, generator=g).to(torch.bfloat16)
+    out = torch.empty(n, 1, hd, dtype=torch.bfloat16, device=DEV)
+    ws = torch.empty(ops.tree_attention_workspace(cache, 1, n), dtype=torch.uint8, device=DEV)
+    y = f.to(DEV)
+    ops.tree_attention(cache, y[:, :1], y[:, 1:2], y[:, 2:], out, _i32([0, n]), None, _i32([24]), n, ws)
+    _check_attention(dict(H=1, Hkv=1, hd=hd, nodes=nodes, ctx=[24], bt=bt, page=page, k=k, v=v, ks=ks, vs=vs, fused=f, parents=[None], scale=hd ** -0.5,
+                          null_self=False, out=out, lse=None))
 
 
 def test_host_memory_is_refused():

@@ -637,8 +637,8 @@ template <int HD> struct TcCfg {
   static constexpr int TILE_BYTES = 128 * HD * 2;
   static constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + 2 * TILE_BYTES, OFF_INFO = OFF_V + 2 * TILE_BYTES;
   static constexpr int INFO_BYTES = 2 * 128 * 4 + 16;                     // key scales, value scales, valid positions (a word for 32)
-  static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2 loader groups][2][128] byte offsets of rows
-  static constexpr int OFF_ML = OFF_ROW + 4 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
+  static constexpr int OFF_ROW = OFF_INFO + INFO * INFO_BYTES;            // [2 loader groups][3][128] byte offsets of rows
+  static constexpr int OFF_ML = OFF_ROW + 6 * 128 * 8;                    // [2][128][2] maxima and sums of the streams
   static constexpr int OFF_PAR = OFF_ML + 2 * 128 * 2 * 4;                // parents
   static constexpr int OFF_ANC = OFF_PAR + MAX_NODES * 2;                 // [MAX_NODES / 32][256] ancestors-or-self of the rows' nodes
   static constexpr int OFF_QF = OFF_ANC + MAX_NODES / 32 * 256 * 4;       // [256] factors of the rows of q
@@ -735,7 +735,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     const int t = threadIdx.x & 127, bar = vals ? 3 : 2;
     constexpr int ES = CODE == PCPB_BF16 ? 2 : 1, PIECES = HD * ES / 16, NP = PIECES;          // 16-byte pieces of a row = pieces of a thread per tile
     constexpr int PB = HD / 8;                                  // pieces of a node's row (bf16)
-    long long* rowoff = reinterpret_cast<long long*>(gen + Cfg::OFF_ROW) + (vals ? 256 : 0);
+    long long* rowoff = reinterpret_cast<long long*>(gen + Cfg::OFF_ROW) + (vals ? 384 : 0);
     const uint8_t* const pages = (const uint8_t*)(vals ? A.c.v : A.c.k);
     const bf16* const nodes = (const bf16*)(vals ? A.a.v : A.a.k);
     const long long node_row = vals ? A.a.v_row : A.a.k_row, node_head = vals ? A.a.v_head : A.a.k_head;
@@ -796,11 +796,14 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       Entry e1 = look(g.t0), e2 = look(g.t0 + 1);
       Found f0 = find(e1), f1 = find(e2);                       // of this tile and the next
       e2 = look(g.t0 + 2);
-      rowoff[(gi & 1) * 128 + t] = f0.off;
+      // Three places of row offsets: at tile i a thread writes those of tile i + 1, while others may still be reading tile i - 1's (they are
+      // only known to have passed tile i - 1's barrier).
+      int slot = gi % 3;
+      rowoff[slot * 128 + t] = f0.off;
       bar_sync(bar, 128);
       if (CODE != PCPB_BF16 && g.t0 < g.ct) {
 #pragma unroll
-        for (int k = 0; k < NP; ++k) cur[k] = piece(k, gi & 1);
+        for (int k = 0; k < NP; ++k) cur[k] = piece(k, slot);
       }
 #pragma unroll 1
       for (int i = 0; i < nt; ++i, ++gi) {
@@ -819,8 +822,9 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
             mbar_arrive(ifull(in));
           }
         }
-        // the next tile's rows, and the pages of the one after
-        if (i + 1 < nt) { rowoff[(st ^ 1) * 128 + t] = f1.off; }
+        // the next tile's rows
+        const int slot1 = slot == 2 ? 0 : slot + 1;
+        if (i + 1 < nt) rowoff[slot1 * 128 + t] = f1.off;
         bar_sync(bar, 128);
         const uint32_t dst = dst0 + st * Cfg::TILE_BYTES, full = full0 + 8u * st;
         wait_empty(empty0 + 8u * st, ((gi >> 1) & 1) ^ 1);
@@ -828,7 +832,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
 #pragma unroll
           for (int k = 0; k < NP; ++k) {
             const int idx = t + 128 * k, row = idx / PIECES, c = idx % PIECES;
-            const long long o = rowoff[st * 128 + row];
+            const long long o = rowoff[slot * 128 + row];
             cp_async16z(dst + sw_off(row, c), pages + (o < 0 ? 0 : o + c * 16), o >= 0);
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
@@ -861,7 +865,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           // their scoreboards, and every use then waits for the newest load (1000 cycles a piece).
           if (more) {
 #pragma unroll
-            for (int k = 0; k < NP; ++k) cur[CODE == PCPB_BF16 ? 0 : k] = piece(k, st ^ 1);
+            for (int k = 0; k < NP; ++k) cur[CODE == PCPB_BF16 ? 0 : k] = piece(k, slot1);
           }
         } else {
           // rows of the nodes (bf16); values that are not numbers are left out and their nodes marked
@@ -911,6 +915,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
           mbar_arrive(full);
         }
         f0 = f1; f1 = find(e2); e2 = look(tile + 3);
+        slot = slot1;
       }
       w += nt;
     }
@@ -1284,9 +1289,11 @@ template <int HD, int CODE> cudaError_t launch_tc(cudaStream_t st, const AttnArg
   e = cudaGetLastError();
   return e == cudaSuccess ? launch_join<HD, TR>(st, A, blocks) : e;
 }
-// Rows of a kv head from which on the tensor-core kernel takes over
-constexpr int TC_FROM = 9;
-bool use_tc(const pcpb_kv_cache& c, int G, int max_nodes) { return c.head_dim != 32 && max_nodes * G >= TC_FROM; }
+// Rows of a kv head from which on the tensor-core kernel takes over.  Its time hardly depends on the rows (up to 128), the other one's grows
+// with every 8.  16 sequences of 4096, 8 kv heads x 128, this kernel against the other: bf16 8 rows 63 / 58 us, 12 rows 64 / 99; e4m3 16 rows
+// 97 / 81, 24 rows 98 / 99, 32 rows 99 / 135.
+constexpr int TC_FROM_BF16 = 9, TC_FROM_CODES = 25;
+bool use_tc(const pcpb_kv_cache& c, int G, int max_nodes) { return c.head_dim != 32 && max_nodes * G >= (c.dtype == PCPB_BF16 ? TC_FROM_BF16 : TC_FROM_CODES); }
 template <int HD, int CODE> cudaError_t launch_any(cudaStream_t st, const AttnArgs& A, int blocks) {
   if constexpr (HD != 32)
     if (use_tc(A.c, A.G, A.a.max_nodes)) return launch_tc<HD, CODE>(st, A, blocks);

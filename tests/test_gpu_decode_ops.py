@@ -488,6 +488,22 @@ def test_first_call_inside_a_capture_and_calls_without_nodes():
     assert torch.equal(s["out"], want)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "i8"])
+@pytest.mark.parametrize("hd,G,nodes,tree", [(128, 4, 24, "tree"), (128, 4, 64, "tree"), (64, 1, 130, "chain"), (128, 4, 1, "chain")])
+def test_the_same_bits_over_many_runs(kind, hd, G, nodes, tree):
+    """Many tiles a block and several blocks an item, run a hundred times: a race between the roles of a block would show as another result
+    now and then."""
+    s = _attention_case(hd, kind, G, 4, 16, [nodes] * 6, [3000, 2900, 1700, 2500, 40, 2222], tree, lse=False)
+    want = s["out"].clone()
+    for _ in range(100):
+        s["out"].fill_(3.0)
+        ops.tree_attention(*s["args"], **s["kw"])
+        assert torch.equal(s["out"], want)
+    s["nodes"], s["ctx"], s["parents"] = s["nodes"][:1], s["ctx"][:1], s["parents"][:1]          # and the first sequence against 64 bits
+    s["out"] = torch.cat([s["out"][:nodes], s["out"][-3:]])
+    _check_attention(s)
+
+
 def test_two_calls_at_once_share_the_inputs():
     """Two streams, one cache and one set of inputs, two outputs and workspaces."""
     for case in ((128, "e4m3", 4, 2, 16, [1, 1, 1], [3000, 2000, 50], "chain"), (128, "bf16", 4, 2, 16, [24, 9, 17], [900, 2000, 50], "tree")):

@@ -160,8 +160,10 @@ __device__ __forceinline__ int seq_at(const long long* plan, int batch, long lon
 // same assignment, and which output columns a lane holds does not matter as long as they are stored where they belong; so no element
 // changes lanes, and a lane reads back from shared memory only what it copied there itself.  Values are paired by position with
 // byte permutes, the weights change from accumulator to operand with movmatrix.
-// Bound: HBM, with the widening of 8-bit codes close behind.  Every warp keeps a ring of units in flight with cp.async (130 to 200 KB an
-// SM); the block-table entries are read one unit ahead of that.
+// Bound: the widening of 8-bit codes (16 sequences of 8192 e4m3 positions, 32 q / 8 kv heads x 128: 64 us, DRAM 41 %, ALU pipe 48 %); HBM
+// for bf16.  Every warp keeps a ring of units in flight with cp.async (130 to 200 KB an SM); the block-table entries are read one unit
+// ahead of that.  With 16 rows a tile, keys as the other operand and loads straight into registers the same case took 131 us, with the
+// ring 101, with 8 rows a tile and sixteen warps 76, with the keys in f16 68.
 constexpr int RW = 8;                // rows of a tile
 
 template <int HD, int CODE> struct Frag {
@@ -625,8 +627,10 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
 //                       otherwise, and a warp of its own for it would cost the loaders the registers that hold their codes.
 // The reference maximum of a row moves only when a score passes it by 2^8 (weights up to 256 cost nothing: bf16 keeps its relative
 // precision), so the output is rescaled in few tiles.
-// Loops over a tile's columns are not unrolled further than 64: with everything unrolled the five roles' code did not fit the instruction
+// Loops over a tile's columns are not unrolled further than 32: with everything unrolled the roles' code did not fit the instruction
 // caches (a third of the stalls were missing instructions).
+// Bound: the softmax warps' issue latency.  64 drafts on 4 sequences of 40960 i8 positions, 32 q / 8 kv heads x 128: 280 us (500 TFLOP/s,
+// tensor pipe 23 %; with one group of loaders and a warp of its own for the products 551); 24 drafts on 16 x 2048 in bf16: 43 us.
 // Every wait is bounded.  A wait that runs out marks the block as failed and sets PCPB_OPS_STUCK; from there on waits return at once and all
 // warps run their loops to the end (the same barriers, valid addresses, wrong numbers), so that nothing hangs.
 constexpr int TR = 256;              // rows of an item

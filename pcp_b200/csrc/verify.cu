@@ -8,8 +8,7 @@
 // (304 KB at 151936 words): a cluster of up to 16 blocks takes a sequence, every warp a contiguous segment of the row.  Per step the warps'
 // maxima and sums go to all blocks of the cluster through distributed shared memory, and after ONE cluster barrier every thread
 // makes the same decision from the same numbers; buffers alternate, so the next exchange needs no second barrier.  32 trees of 24 tokens at
-// 151936 words: 67 us (one block a sequence: 519).  Where all rows together are small (AHEAD_BYTES) they are read before the walk, four at
-// a time, and a step is a decision only: 16 chains of 8 at 65536 f32 words take 52 us.
+// 151936 words: 67 us (one block a sequence: 519).  Rows of short chains (AHEAD_N) are read before the walk, four at a time, and a step is a decision only: 16 chains of 8 at 65536 f32 words take 52 us.
 //
 // Precision.  Sums of a step are f32.  S is off (relative) by at most 2^-22 of exp2, three roundings of its argument, whose weighted mean
 // is at most log2 V (3 ln 2 log2(V) 2^-24 = 2.1e-6), as much again and 2^-22 for each of the dozen joins of parts, and the
@@ -30,8 +29,10 @@ constexpr int VW = 8, VT = 32 * (VW + 1);          // warps that read rows, thre
 constexpr int MAX_CL = 16;                         // blocks of a cluster
 constexpr int MAX_N = PCPB_TREE_MAX_NODES;
 constexpr int KEEP = 10;                           // a lane's first pieces of the last token's row, whose sums are kept for the search
-constexpr int AHEAD_N = 64;                        // most nodes whose rows are all read ahead of the walk
-constexpr double AHEAD_BYTES = 32e6;
+constexpr int AHEAD_N = 8;                         // most nodes whose rows are all read ahead of the walk
+// Reading every row before the walk pays where most of them will be walked anyway.  Ahead / one after the other: 1 chain of 6 at 50304 words 15 /
+// 21 us, 32 chains of 8 at 50304 45 / 48, 16 of 8 at 65536 (f32, drafter) 52 / 54; but 1 tree of 24 at 151936 68 / 36, 16 at 65536 68 / 43.
+constexpr double AHEAD_BYTES = 64e6;
 
 struct VerifyArgs {
   pcpb_verify v;
@@ -534,7 +535,7 @@ extern "C" int pcpb_op_verify_drafts(void* stream, const pcpb_verify* args, int3
   d.on(status, "status");
   if (d.enter()) return d.rc;
   const bool greedy = v.temperature < 1e-6, half = v.dtype == PCPB_BF16;
-  A.ahead = (double)v.n_rows * v.vocab * (half ? 2 : 4) <= AHEAD_BYTES;
+  A.ahead = v.max_nodes <= AHEAD_N && (double)v.n_rows * v.vocab * (half ? 2 : 4) <= AHEAD_BYTES;
   cudaStream_t st = (cudaStream_t)stream;
   return d.done(half ? (greedy ? launch<bf16, true>(st, A) : launch<bf16, false>(st, A)) : (greedy ? launch<float, true>(st, A) : launch<float, false>(st, A)));
 }

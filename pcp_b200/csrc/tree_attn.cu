@@ -8,8 +8,8 @@
 //
 // Work.  The rows of one item are those of a sequence's nodes and of the query heads of one kv head, node-major (row = node G + head),
 // in tiles of ROWS; its keys are the cached positions, then the nodes, in tiles of TILE.  All tiles of all items are laid end
-// to end, and block c of the grid takes the c-th equal share of them: ragged contexts balance, and one long context spreads
-// over the whole GPU.  Lengths are read on the device, so the grid does not depend on them.  An item that lies in one block is
+// to end, and block c of the grid takes the c-th equal share of them (or one whole item: make_plan): ragged contexts balance, and one
+// long context spreads over the whole GPU.  Lengths are read on the device, so the grid does not depend on them.  An item that lies in one block is
 // finished there; the parts of the others go to the workspace (a block has at most two of them: the item it begins in and the
 // one it ends in) and k_tree_join adds them up in block order, so results do not depend on timing.
 #include <cuda_fp8.h>
@@ -25,6 +25,7 @@ namespace {
 
 constexpr int TILE = 128;            // keys of a scheduling step
 constexpr int MAX_NODES = PCPB_TREE_MAX_NODES, MAX_BATCH = PCPB_TREE_MAX_BATCH;
+constexpr int SLACK_FEW = 2, SLACK_MANY = 6;      // make_plan: what a segment and the join cost, in tiles of either kernel
 constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -32,7 +33,7 @@ struct AttnArgs {
   pcpb_tree_attn a;
   int32_t* status;
   int G;                             // query heads of a kv head
-  long long* plan;                   // workspace: [batch + 1] first tile of every sequence
+  long long* plan;                   // workspace: [batch + 2] first tile of every sequence, all tiles, pitch
   float* part_ml;                    // [blocks][2][ROWS][2] maximum and sum
   float* part_o;                     // [blocks][2][ROWS][HD]
 };
@@ -120,17 +121,42 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& A, int b) {
 }
 __device__ __forceinline__ int tiles_of(int x) { return (x + TILE - 1) / TILE; }
 
-// plan[b] = first tile of sequence b, plan[batch] = all tiles; by the whole block, into shared memory.
-template <int ROWS> __device__ void make_plan(const AttnArgs& A, long long* plan) {
-  __shared__ long long wsum[32];
+// plan[b] = first tile of sequence b, plan[batch] = all tiles, plan[batch + 1] = pitch; by the whole block, into shared memory.
+// pitch > 0: every block takes one whole item, whose tiles are counted as `pitch` of them (the longest item's).  That is the better cut where
+// there are no more items than blocks and the longest is at most `slack` tiles above the equal share, because a second segment of a block
+// (rows of q, outputs, filling the pipeline) and the join cost about that many.  24 drafts on 16 sequences of 2048 (bf16): 49 us cut
+// into equal shares, 43 with whole items; chains of 130 on 8 sequences of 1000, 16 heads x 64: 58 and 47.
+template <int ROWS> __device__ void make_plan(const AttnArgs& A, long long* plan, int slack) {
+  __shared__ long long wsum[32], wtiles[32];
+  __shared__ int witems[32], wmost[32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  long long tiles = 0;
+  int items = 0, most = 0;
+  for (int b = threadIdx.x; b < A.c.batch; b += blockDim.x) {
+    const Seq s = seq_of(A, b);
+    const int T = tiles_of(s.ctx) + tiles_of(s.n), n = (s.n * A.G + ROWS - 1) / ROWS * A.c.n_kv_head;
+    tiles += (long long)n * T;
+    items += n;
+    if (n) most = max(most, T);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    items += __shfl_xor_sync(0xffffffffu, items, o);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if (lane == 0) { wtiles[w] = tiles; witems[w] = items; wmost[w] = most; }
+  __syncthreads();
+  tiles = 0; items = 0; most = 0;
+  for (int i = 0; i < nw; ++i) { tiles += wtiles[i]; items += witems[i]; most = max(most, wmost[i]); }
+  const int pitch = items <= (int)gridDim.x && most <= tile_share(tiles, gridDim.x) + slack ? most : 0;
   long long base = 0;
   for (int b0 = 0; b0 < A.c.batch; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
     long long x = 0;
     if (b < A.c.batch) {
       const Seq s = seq_of(A, b);
-      x = (long long)((s.n * A.G + ROWS - 1) / ROWS) * A.c.n_kv_head * (tiles_of(s.ctx) + tiles_of(s.n));
+      x = (long long)((s.n * A.G + ROWS - 1) / ROWS) * A.c.n_kv_head * (pitch ? pitch : tiles_of(s.ctx) + tiles_of(s.n));
     }
     long long inc = x;
 #pragma unroll
@@ -143,8 +169,12 @@ template <int ROWS> __device__ void make_plan(const AttnArgs& A, long long* plan
     base = all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) plan[A.c.batch] = base;
+  if (threadIdx.x == 0) { plan[A.c.batch] = base; plan[A.c.batch + 1] = pitch; }
   __syncthreads();
+}
+// Tiles of a block's share
+__device__ __forceinline__ long long share_of(const long long* plan, int batch, int blocks) {
+  return plan[batch + 1] ? plan[batch + 1] : tile_share(plan[batch], blocks);
 }
 // The sequence tile t belongs to: plan[b] <= t < plan[b + 1]
 __device__ __forceinline__ int seq_at(const long long* plan, int batch, long long t) {
@@ -373,8 +403,8 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
   typedef Ring<HD, CODE> G;
   constexpr int WARPS = F::WARPS;
   extern __shared__ __align__(16) uint8_t smem[];
-  long long* plan = reinterpret_cast<long long*>(smem);                       // [batch + 1]
-  uint8_t* rings = smem + ((A.c.batch + 1) * 8 + 15) / 16 * 16;
+  long long* plan = reinterpret_cast<long long*>(smem);                       // [batch + 2]
+  uint8_t* rings = smem + ((A.c.batch + 2) * 8 + 15) / 16 * 16;
   __shared__ float mml[WARPS][RW][2];
   __shared__ int16_t par[MAX_NODES];
   __shared__ uint32_t anc[RW][MAX_NODES / 32];
@@ -383,16 +413,17 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
   float* const mine = reinterpret_cast<float*>(ring);           // [RW][HD]
   const uint32_t ring_s = smem_u32(ring);
   pdl_launch_dependents();
-  make_plan<RW>(A, plan);
-  const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
-  if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
+  make_plan<RW>(A, plan, SLACK_FEW);
+  const long long total = plan[A.c.batch], per = share_of(plan, A.c.batch, gridDim.x);
+  if (blockIdx.x == 0) for (int b = threadIdx.x; b < A.c.batch + 2; b += blockDim.x) A.plan[b] = plan[b];
   const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
   for (long long w = w0; w < w1;) {
     const int b = seq_at(plan, A.c.batch, w);
     const Seq s = seq_of(A, b);
     const int ct = tiles_of(s.ctx), T = ct + tiles_of(s.n), RT = (s.n * A.G + RW - 1) / RW;
-    const long long at = w - plan[b], item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)T) : at / T;
-    const int t0 = (int)(at - item * T), t1 = (int)min((long long)T, t0 + (w1 - w));
+    const int pitch = (int)plan[A.c.batch + 1], P = pitch ? pitch : T;
+    const long long at = w - plan[b], item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)P) : at / P;
+    const int t0 = (int)(at - item * P), t1 = (int)min((long long)T, t0 + (w1 - w));
     const int kvh = (int)item / RT, row0 = ((int)item - kvh * RT) * RW, rows = s.n * A.G;
     RowState<HD> R;
 #pragma unroll
@@ -560,7 +591,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(Frag<HD, CODE>::WA
       }
     }
     __syncthreads();
-    w += t1 - t0;
+    w = pitch ? w1 : w + (t1 - t0);
   }
 }
 
@@ -575,6 +606,7 @@ template <int HD, int ROWS> __global__ void __launch_bounds__(256) k_tree_join(c
   if (item >= RT * A.c.n_kv_head) return;
   const int kvh = item / RT, row0 = item % RT * ROWS, r0 = blockIdx.z * 16;
   if (row0 + r0 >= rows) return;
+  if (A.plan[A.c.batch + 1]) return;                            // whole items: nothing was split
   const Parts P = parts_of(A.plan[b] + (long long)item * T, T, tile_share(A.plan[A.c.batch], blocks));
   if (P.c0 == P.c1) return;
   for (int i = threadIdx.x; i < 16 * (HD / 4); i += blockDim.x) {
@@ -648,7 +680,7 @@ template <int HD> struct TcCfg {
   static constexpr int OFF_QF = OFF_ANC + MAX_NODES / 32 * 256 * 4;       // [256] factors of the rows of q
   static constexpr int OFF_BAR = OFF_QF + 256 * 4;
   static constexpr int OFF_PLAN = OFF_BAR + 256;
-  static constexpr int BYTES = OFF_PLAN + (MAX_BATCH + 1) * 8 + 1024;
+  static constexpr int BYTES = OFF_PLAN + (MAX_BATCH + 2) * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory");
 };
 
@@ -670,7 +702,7 @@ __device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, 
 }
 
 // The blocks' segments: a run of tiles [t0, t1) of one item
-struct Seg { int b, kvh, row0, rows, t0, t1, ct, T; Seq s; };
+struct Seg { int b, kvh, row0, rows, t0, t1, ct, T; Seq s; long long next; };       // next: where the block goes on
 __device__ __forceinline__ Seg seg_at(const AttnArgs& A, const long long* plan, long long w, long long w1) {
   Seg g;
   g.b = seq_at(plan, A.c.batch, w);
@@ -678,9 +710,11 @@ __device__ __forceinline__ Seg seg_at(const AttnArgs& A, const long long* plan, 
   g.ct = tiles_of(g.s.ctx); g.T = g.ct + tiles_of(g.s.n);
   const int all = g.s.n * A.G, RT = (all + TR - 1) / TR;
   const long long at = w - plan[g.b];
-  const long long item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)g.T) : at / g.T;
-  g.t0 = (int)(at - item * g.T);
+  const int pitch = (int)plan[A.c.batch + 1], P = pitch ? pitch : g.T;
+  const long long item = at < 0x7fffffffll ? (long long)((unsigned)at / (unsigned)P) : at / P;
+  g.t0 = (int)(at - item * P);
   g.t1 = (int)min((long long)g.T, g.t0 + (w1 - w));
+  g.next = pitch ? w1 : w + (g.t1 - g.t0);
   g.kvh = (int)item / RT; g.row0 = ((int)item - g.kvh * RT) * TR;          // items of a sequence: kv heads x row tiles, an int
   g.rows = min(TR, all - g.row0);
   return g;
@@ -722,13 +756,13 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  make_plan<TR>(A, plan);                                       // (its barriers also publish the setup above)
+  make_plan<TR>(A, plan, SLACK_MANY);                                       // (its barriers also publish the setup above)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
-  const long long total = plan[A.c.batch], per = tile_share(total, gridDim.x);
-  if (blockIdx.x == 0) for (int b = threadIdx.x; b <= A.c.batch; b += blockDim.x) A.plan[b] = plan[b];
+  const long long total = plan[A.c.batch], per = share_of(plan, A.c.batch, gridDim.x);
+  if (blockIdx.x == 0) for (int b = threadIdx.x; b < A.c.batch + 2; b += blockDim.x) A.plan[b] = plan[b];
   const long long w0 = per * blockIdx.x, w1 = min(total, w0 + per);
   auto s_col = [&](int x) { return tmem + 128u * x; };
   auto o_col = [&](int x) { return tmem + 256u + 128u * x; };
@@ -921,7 +955,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
         f0 = f1; f1 = find(e2); e2 = look(tile + 3);
         slot = slot1;
       }
-      w += nt;
+      w = g.next;
     }
     flush();
   } else {
@@ -1224,7 +1258,7 @@ template <int HD, int CODE> __global__ void __launch_bounds__(TC_THREADS, 1) k_t
       bar_sync(1, 256);                                         // the outputs, ml, par and q are used again
       tc_fence_after();
       gi += nt;
-      w += nt;
+      w = g.next;
     }
   }
   tc_fence_before();
@@ -1250,7 +1284,7 @@ Layout layout(const pcpb_kv_cache& c, int blocks, int rows_tile) {
   Layout L;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   L.plan = 0;
-  L.ml = up((size_t)(c.batch + 1) * 8);
+  L.ml = up((size_t)(c.batch + 2) * 8);
   L.o = L.ml + up((size_t)blocks * 2 * rows_tile * 2 * 4);
   L.bytes = L.o + up((size_t)blocks * 2 * rows_tile * c.head_dim * 4);
   return L;
@@ -1276,9 +1310,9 @@ template <int HD, int ROWS> cudaError_t launch_join(cudaStream_t st, const AttnA
   return cudaLaunchKernelEx(&cfg, k_tree_join<HD, ROWS>, A, blocks);
 }
 template <int HD, int CODE> cudaError_t launch_rows(cudaStream_t st, const AttnArgs& A, int blocks) {
-  const size_t smem = ((size_t)(A.c.batch + 1) * 8 + 15) / 16 * 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
+  const size_t smem = ((size_t)(A.c.batch + 2) * 8 + 15) / 16 * 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
   static bool done[64] = {};
-  const size_t most = (MAX_BATCH + 1) * 8 + 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
+  const size_t most = (MAX_BATCH + 2) * 8 + 16 + (size_t)Frag<HD, CODE>::WARPS * Ring<HD, CODE>::BYTES;
   cudaError_t e = allow_smem(k_tree_rows<HD, CODE>, done, most);
   if (e != cudaSuccess) return e;
   k_tree_rows<HD, CODE><<<blocks, Frag<HD, CODE>::WARPS * 32, smem, st>>>(A);

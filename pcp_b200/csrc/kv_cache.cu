@@ -25,8 +25,9 @@ struct KvArgs {
 template <int CODE> struct CodeMax { static constexpr float v = CODE == PCPB_I8 ? 127.f : 448.f; };
 
 // x / a rounded to nearest, from the correctly rounded reciprocal r of a: one product and one correction (P. Markstein, "Computation of
-// elementary functions on the IBM RISC System/6000 processor", 1990, theorem on the last step of a division).  The remainder must not
-// fall below the smallest number: callers keep to a >= 2^-100, where it does so only for quotients that round to code 0.
+// elementary functions on the IBM RISC System/6000 processor", 1990, theorem on the last step of a division).  The remainder, a
+// multiple of 2^-46 times the powers of two of quotient and divisor, must not fall below the smallest number, 2^-149: callers keep to
+// a >= 2^-80, where it does so only for quotients below 2^-23, which become code 0.
 __device__ __forceinline__ float quotient(float x, float a, float r) {
   const float q = x * r;
   return fmaf(fmaf(-q, a, x), r, q);
@@ -34,7 +35,7 @@ __device__ __forceinline__ float quotient(float x, float a, float r) {
 // Eight values to eight codes (two 32-bit words).
 template <int CODE> __device__ __forceinline__ uint2 encode8(const float (&f)[8], float a) {
   float y[8];
-  if (a >= 7.9e-31f) {
+  if (a >= 8.28e-25f) {
     const float r = __frcp_rn(a);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = quotient(f[i], a, r);

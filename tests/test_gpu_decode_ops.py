@@ -119,6 +119,24 @@ def test_a_row_with_an_infinity_or_nan_reads_back_as_nan(kind):
     assert torch.equal(out.isnan(), bad[..., None].expand_as(out))
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "i8"])
+def test_codes_of_rows_of_every_size(kind):
+    """f32 rows from 2^-140 to 2^120, on both sides of every switch in the quotient, with elements across 40 powers of two: codes and scales bit
+    for bit those of f32 divisions."""
+    g = torch.Generator().manual_seed(11)
+    n, page, hd = 261, 16, 64
+    x = torch.randn(n, 2, hd, generator=g).double() * torch.exp2(-40 * torch.rand(n, 2, hd, generator=g).double())
+    x = (x * torch.exp2(torch.arange(n).double() - 140)[:, None, None]).float()
+    k, v, ks, vs, _, _ = _cache(kind, 17, 1, page, hd)
+    cache = ops.KvCache(k, v, torch.arange(17, dtype=I32, device=DEV)[None], ks, vs)
+    d = x.to(DEV)
+    ops.kv_write(cache, d[:, :1], d[:, 1:], _i32([0, n]), _i32([0]), n)
+    for i, (pages, scales) in enumerate(((k, ks), (v, vs))):
+        c, a = ref.quantise(x[:, i], kind)
+        assert torch.equal(scales.cpu().flatten()[:n], a)
+        assert torch.equal(_raw(pages).cpu().reshape(-1, hd)[:n], _raw(c))
+
+
 def test_index_lists_bad_pages_and_bad_positions():
     """index picks source rows and leaves entries out; entries of pages outside the cache or positions outside the table are left out (written)
     or zero (read), and say so."""

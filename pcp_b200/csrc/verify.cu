@@ -8,7 +8,7 @@
 // (304 KB at 151936 words): a cluster of up to 16 blocks takes a sequence, every warp a contiguous segment of the row.  Per step the warps'
 // maxima and sums go to all blocks of the cluster through distributed shared memory, and after ONE cluster barrier every thread
 // makes the same decision from the same numbers; buffers alternate, so the next exchange needs no second barrier.  32 trees of 24 tokens at
-// 151936 words: 67 us (one block a sequence: 519).  Rows of short chains (AHEAD_N) are read before the walk, four at a time, and a step is a decision only: 16 chains of 8 at 65536 f32 words take 52 us.
+// 151936 words: 65 to 72 us over several runs (one block a sequence: 519).  Rows of short chains (AHEAD_N) are read before the walk, four at a time, and a step is a decision only: 16 chains of 8 at 65536 f32 words take 52 to 59 us.
 //
 // Precision.  Sums of a step are f32.  S is off (relative) by at most 2^-22 of exp2, three roundings of its argument, whose weighted mean
 // is at most log2 V (3 ln 2 log2(V) 2^-24 = 2.1e-6), as much again and 2^-22 for each of the dozen joins of parts, and the
